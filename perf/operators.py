@@ -167,10 +167,10 @@ def _quantize(x, fmt):
         byte, scale, row = (e + 127).to(torch.uint8), _power(e), None
         full = scale.double()
     else:
-        # row: the smallest power of two (at least 2^-126) with amax_row / 6 <= 448 * row
+        # row: the smallest power of two (at least 2^-100) with amax_row / 6 <= 448 * row
         top = amax.amax(-1)
         m, e = torch.frexp(top)
-        row = _power(torch.where(top > 0, (e - 11 - (m <= 0.65625).int()).clamp(min=-126), torch.zeros_like(e)))
+        row = _power(torch.where(top > 0, (e - 11 - (m <= 0.65625).int()).clamp(min=-100), torch.zeros_like(e)))
         fp8 = (amax.double() / (6.0 * row.double()[:, None])).float().to(torch.float8_e4m3fn)
         byte, scale = fp8.view(torch.uint8), fp8.float()
         full = scale.double() * row.double()[:, None]
@@ -411,7 +411,7 @@ def _exact_quantize(x, fmt):
         peak = top.amax(1, keepdim=True)
         e = torch.ceil(torch.log2(peak.clamp(min=2.0 ** -149) / 2688.0))
         e = torch.where(peak <= 2688.0 * torch.exp2(e - 1), e - 1, e)  # log2 is rounded: one step either way
-        e = torch.where(peak > 2688.0 * torch.exp2(e), e + 1, e).clamp(min=-126)
+        e = torch.where(peak > 2688.0 * torch.exp2(e), e + 1, e).clamp(min=-100)
         row = torch.where(peak > 0, torch.exp2(e), row)
         want = top / (6.0 * row)
         # nearest E4M3: steps of 2^(exponent - 3), 2^-9 below 2^-6; round() takes ties to even
