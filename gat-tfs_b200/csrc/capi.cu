@@ -37,12 +37,19 @@ int tfs_dispatch(const gat_b200_graph* g, const gat_b200_layer* p, const void* x
                  const float* right, const float* max, const float* fixed_p, const float* fixed_den, int rounding,
                  int block, int threshold, int norm, int hidden, void* out, int out_bf16, int ldo, float* den,
                  float* max_out, cudaStream_t st, int* launches);
+int fp4_quantize_launch(int format, uint64_t n, int width, const void* x, int x_dtype, int ldx, void* codes, int ldc,
+                        void* scales, float* row_scale, void* values, int v_dtype, int ldv, cudaStream_t st);
+int fp4_product_launch(int format, uint64_t m, int n, int k, const void* a, int lda, const void* a_scales,
+                       const float* a_row, const void* b, int ldb, const void* b_scales, const float* b_row, void* out,
+                       int out_dtype, int ldo, cudaStream_t st);
+int fp4_check_error();
 int device_check_errors() {
     int rc = projection_tc_check_error();
     int rc2 = aggregate_check_error();
     int rc3 = tfs_tc_check_error();
     int rc4 = peer_check_error();
-    return rc ? rc : (rc2 ? rc2 : (rc3 ? rc3 : rc4));
+    int rc5 = fp4_check_error();
+    return rc ? rc : (rc2 ? rc2 : (rc3 ? rc3 : (rc4 ? rc4 : rc5)));
 }
 
 namespace {
@@ -346,6 +353,21 @@ int gat_b200_projection(const gat_b200_layer* p, uint64_t n, const void* x, int 
                         int h_dtype, int ldh, float* left, float* right, void* stream) {
     clear_error();
     return projection_dispatch(p, n, x, ldx, precision, h, h_dtype, ldh, left, right, as_stream(stream));
+}
+
+int gat_b200_fp4_quantize(int format, uint64_t n, int width, const void* x, int x_dtype, int ldx, void* codes, int ldc,
+                          void* scales, float* row_scale, void* values, int v_dtype, int ldv, void* stream) {
+    clear_error();
+    return fp4_quantize_launch(format, n, width, x, x_dtype, ldx, codes, ldc, scales, row_scale, values, v_dtype, ldv,
+                               as_stream(stream));
+}
+
+int gat_b200_fp4_product(int format, uint64_t m, int n, int k, const void* a, int lda, const void* a_scales,
+                         const float* a_row, const void* b, int ldb, const void* b_scales, const float* b_row,
+                         void* out, int out_dtype, int ldo, void* stream) {
+    clear_error();
+    return fp4_product_launch(format, m, n, k, a, lda, a_scales, a_row, b, ldb, b_scales, b_row, out, out_dtype, ldo,
+                              as_stream(stream));
 }
 
 int gat_b200_projection_scatter(const gat_b200_layer* p, uint64_t n, const void* x, int ldx, void* h, int ldh,

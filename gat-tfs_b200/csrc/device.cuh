@@ -2,6 +2,7 @@
 #pragma once
 #include <cuda_runtime.h>
 #include <cstdint>
+#include <initializer_list>
 
 #include "gat_b200_internal.h"
 
@@ -24,6 +25,10 @@ int cuda_fail(cudaError_t e, const char* what);
         cudaError_t _e = cudaGetLastError();                     \
         if (_e != cudaSuccess) return ::gatb::cuda_fail(_e, what); \
     } while (0)
+
+// GAT_B200_EINVAL unless every non-null pointer is memory of the current device
+// (device or managed): refused here, it cannot fault inside a kernel.
+int check_device_pointers(const char* what, std::initializer_list<const void*> ptrs);
 
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 

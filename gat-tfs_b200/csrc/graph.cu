@@ -25,6 +25,20 @@ int cuda_fail(cudaError_t e, const char* what) {
     return fail_code(GAT_B200_ECUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
+int check_device_pointers(const char* what, std::initializer_list<const void*> ptrs) {
+    int dev = 0;
+    GATB_CUDA(cudaGetDevice(&dev));
+    for (const void* p : ptrs) {
+        if (!p) continue;
+        cudaPointerAttributes at{};
+        GATB_CUDA(cudaPointerGetAttributes(&at, p));
+        if ((at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) ||
+            (at.type == cudaMemoryTypeDevice && at.device != dev))
+            return fail(std::string(what) + ": a pointer is not memory of the current device");
+    }
+    return 0;
+}
+
 namespace {
 
 int dalloc(void** p, size_t bytes, const char* what) {

@@ -53,6 +53,17 @@ int gat_b200_padded_ld(int width, int elem_dtype) {
     return gatb::padded_ld(width, elem_dtype == GAT_B200_BF16 ? 2 : 4);
 }
 
+int gat_b200_fp4_ld(int width) {
+    if (width <= 0 || width > (1 << 24)) return 0;
+    return (width + 31) / 32 * 16;
+}
+
+uint64_t gat_b200_fp4_scale_bytes(int format, uint64_t n, int width) {
+    if ((format != GAT_B200_MXFP4 && format != GAT_B200_NVFP4) || width <= 0 || width > (1 << 24)) return 0;
+    const uint64_t cols = format == GAT_B200_MXFP4 ? 128 : 64;  // columns of a scale tile
+    return (n + 127) / 128 * ((uint64_t(width) + cols - 1) / cols) * 512;
+}
+
 uint16_t gat_b200_rne(float x) {
     uint32_t u;
     std::memcpy(&u, &x, 4);

@@ -438,6 +438,26 @@ int make_row_gather_map(CUtensorMap* m, const void* base, uint64_t cols, uint64_
     return 0;
 }
 
+// Tensor map of up to three dimensions (innermost first; strides in bytes of
+// dimensions 1 and up), 128-byte swizzle or none, zeros outside.
+int make_tiled_map(CUtensorMap* m, int type, int rank, const void* base, const uint64_t* dims, const uint64_t* strides,
+                   const uint32_t* box, bool swizzle) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail_code(GAT_B200_ECUDA, "cuTensorMapEncodeTiled unavailable");
+    cuuint64_t d[3], st[2];
+    cuuint32_t b[3], estr[3] = {1, 1, 1};
+    for (int i = 0; i < rank; ++i) {
+        d[i] = dims[i];
+        b[i] = box[i];
+        if (i) st[i - 1] = strides[i - 1];
+    }
+    CUresult r = fn(m, CUtensorMapDataType(type), cuuint32_t(rank), const_cast<void*>(base), d, st, b, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail_code(GAT_B200_ECUDA, "cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
+    return 0;
+}
+
 // Returns GAT_B200_EUNSUPPORTED when the shape is outside the kernel (the
 // caller then uses the CUDA-core projection).
 // max_ctas > 0 caps the persistent grid (the multi-GPU forward runs this

@@ -92,6 +92,48 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                  : "memory");
 }
+// Instruction descriptor of kind::mxf4 / mxf4nvf4 (E2M1 A/B, both K-major, FP32
+// D): scale bytes E8M0 or E4M3, taken from byte `sf` (0..3) of each scale word.
+__host__ __device__ constexpr uint32_t idesc_fp4(int M, int N, int e8m0, int sf) {
+    return (uint32_t(sf) << 4) | (1u << 7) | (1u << 10) | (uint32_t(N >> 3) << 17) | (uint32_t(e8m0) << 23) |
+           (uint32_t(M >> 4) << 24) | (uint32_t(sf) << 29);
+}
+// 4-bit block-scaled MMA of K = 64: E8M0 scales per 32 or E4M3 scales per 16
+// elements, in tensor memory at sfa / sfb (32 rows per column). CG: CTAs of the group.
+template <bool E8M0, int CG>
+__device__ __forceinline__ void mma_fp4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
+                                        uint32_t sfb, uint32_t accumulate) {
+#define GATB_MMA_FP4(CGS, KIND)                                                                      \
+    asm volatile(                                                                                     \
+        "{\n\t.reg .pred p;\n\t"                                                                      \
+        "setp.ne.b32 p, %6, 0;\n\t"                                                                   \
+        "tcgen05.mma.cta_group::" CGS ".kind::" KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(  \
+            tmem_d),                                                                                  \
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                       \
+        : "memory")
+    if constexpr (E8M0 && CG == 1)
+        GATB_MMA_FP4("1", "mxf4.block_scale.scale_vec::2X");
+    else if constexpr (E8M0)
+        GATB_MMA_FP4("2", "mxf4.block_scale.scale_vec::2X");
+    else if constexpr (CG == 1)
+        GATB_MMA_FP4("1", "mxf4nvf4.block_scale.scale_vec::4X");
+    else
+        GATB_MMA_FP4("2", "mxf4nvf4.block_scale.scale_vec::4X");
+#undef GATB_MMA_FP4
+}
+// 512 bytes of shared memory (32 rows of 16 bytes) to 4 columns of tensor
+// memory, the same in all four lane quarters.
+template <int CG>
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+    if constexpr (CG == 1)
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Descriptor of such a tile: no swizzle, 8-row groups of 128 bytes.
+__device__ __forceinline__ uint64_t desc_scales(uint32_t saddr) {
+    return uint64_t((saddr >> 4) & 0x3fff) | (uint64_t(1) << 16) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
+}
 // 32 lanes x 8 / 16 consecutive FP32 columns; load and wait in one statement so
 // no use of the registers can be scheduled before the wait.
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, float* v) {
@@ -117,6 +159,23 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
         : "memory");
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+// 32 lanes x 32 consecutive FP32 columns, load and wait in one statement.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 // 32 lanes x 64 consecutive FP32 columns, load and wait in one statement.
 __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* v) {
@@ -148,6 +207,12 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
         ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y)
         : "memory");
+}
+// Untiled copy global -> shared: addresses and size multiples of 16 bytes.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
 }
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"

@@ -29,6 +29,7 @@ if not LIB_PATH.exists():
 _lib = C.CDLL(str(LIB_PATH))
 
 F32, BF16 = 0, 1
+MXFP4, NVFP4 = 2, 3
 PATH_STANDARD_BF16, PATH_STANDARD_FP32, PATH_TFS_BF16, PATH_ADAPTIVE_BF16, PATH_MATCHED_ATTENTION = 0, 1, 2, 3, 4
 TFS_EDGE, TFS_BLOCK, TFS_SPLIT = 0, 1, 2
 LR_BF16, LR_FP32 = 0, 1
@@ -78,6 +79,12 @@ SIGNATURES = [
     ("gat_b200_layer_destroy", C.c_int, [_vp]),
     ("gat_b200_convert", C.c_int, [C.c_uint64, C.c_int, _vp, C.c_int, _vp, C.c_int, _vp]),
     ("gat_b200_projection", C.c_int, [_vp, C.c_uint64, _vp, C.c_int, C.c_int, _vp, C.c_int, C.c_int, _vp, _vp, _vp]),
+    ("gat_b200_fp4_ld", C.c_int, [C.c_int]),
+    ("gat_b200_fp4_scale_bytes", C.c_uint64, [C.c_int, C.c_uint64, C.c_int]),
+    ("gat_b200_fp4_quantize", C.c_int, [C.c_int, C.c_uint64, C.c_int, _vp, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp,
+                                        _vp, C.c_int, C.c_int, _vp]),
+    ("gat_b200_fp4_product", C.c_int, [C.c_int, C.c_uint64, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp, _vp, C.c_int,
+                                       _vp, _vp, _vp, C.c_int, C.c_int, _vp]),
     ("gat_b200_max_prescan", C.c_int, [_vp, C.c_int, _vp, _vp, _vp, _vp]),
     ("gat_b200_edge_softmax", C.c_int, [_vp, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     ("gat_b200_standard_aggregate", C.c_int, [_vp, C.c_int, C.c_int, _vp, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp, C.c_int, _vp, _vp, _vp]),
@@ -464,6 +471,29 @@ def projection(layer: DeviceLayer, n, x, ldx, precision, h=None, h_dtype=BF16, l
                stream=None):
     _check(_lib.gat_b200_projection(layer.handle, n, _ptr(x), ldx, precision, _ptr(h), h_dtype, ldh, _ptr(left),
                                     _ptr(right), _stream(stream)))
+
+
+def fp4_ld(width: int) -> int:
+    """Bytes of a 4-bit code row of `width` columns as the library lays it out."""
+    return _lib.gat_b200_fp4_ld(width)
+
+
+def fp4_scale_bytes(fmt: int, n: int, width: int) -> int:
+    """Bytes of the block scales of an n x width table (MXFP4 or NVFP4)."""
+    return _lib.gat_b200_fp4_scale_bytes(fmt, n, width)
+
+
+def fp4_quantize(fmt: int, n, width, x, x_dtype, ldx, codes, ldc, scales, row_scale=None, values=None, v_dtype=BF16,
+                 ldv=0, stream=None):
+    """Rows to a microscaled 4-bit table (gat_b200_fp4_quantize)."""
+    _check(_lib.gat_b200_fp4_quantize(fmt, n, width, _ptr(x), x_dtype, ldx, _ptr(codes), ldc, _ptr(scales),
+                                      _ptr(row_scale), _ptr(values), v_dtype, ldv, _stream(stream)))
+
+
+def fp4_product(fmt: int, m, n, k, a, lda, a_scales, a_row, b, ldb, b_scales, b_row, out, out_dtype, ldo, stream=None):
+    """out = a b^T of two 4-bit tables (gat_b200_fp4_product)."""
+    _check(_lib.gat_b200_fp4_product(fmt, m, n, k, _ptr(a), lda, _ptr(a_scales), _ptr(a_row), _ptr(b), ldb,
+                                     _ptr(b_scales), _ptr(b_row), _ptr(out), out_dtype, ldo, _stream(stream)))
 
 
 PEER_HANDLE_BYTES = 64

@@ -39,6 +39,10 @@ extern "C" {
 #define GAT_B200_F32 0
 #define GAT_B200_BF16 1
 
+/* Formats of 4-bit tables (gat_b200_fp4_quantize). */
+#define GAT_B200_MXFP4 2 /* E2M1, blocks of 32 columns, E8M0 scale */
+#define GAT_B200_NVFP4 3 /* E2M1, blocks of 16 columns, E4M3 scale, FP32 scale per row */
+
 /* Layer paths, named after the reference's --path values
  * (baseline/bench/main.cpp:30, baseline/src/common.cpp:126-134). */
 #define GAT_B200_PATH_STANDARD_BF16 0 /* B0: BF16 X/W on tcgen05, FP32 softmax state */
@@ -222,6 +226,52 @@ int gat_b200_convert(uint64_t n, int width, const float* in, int ld_in, uint16_t
  * left/right FP32 [n][heads]. */
 int gat_b200_projection(const gat_b200_layer* p, uint64_t n, const void* x, int ldx, int precision,
                         void* h, int h_dtype, int ldh, float* left, float* right, void* stream);
+
+/* ---- 4-bit projection (no counterpart in the reference, whose narrowest
+ * product is BF16) -------------------------------------------------------- */
+
+/* A 4-bit table of n rows x width columns:
+ *  codes   E2M1 elements (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives), two
+ *          per byte, the even column in the low half; rows of ldc bytes, of
+ *          which gat_b200_fp4_ld(width) hold the columns and zeros behind them.
+ *  scales  one byte per block of 32 (MXFP4: E8M0) or 16 (NVFP4: E4M3) columns,
+ *          gat_b200_fp4_scale_bytes(format, n, width) bytes: tiles of 128 rows
+ *          x 4 blocks (512 bytes), the tiles of the same 128 rows one after
+ *          another, byte (row % 32) * 16 + (row / 32 % 4) * 4 + block % 4 of
+ *          a tile. The blocks that fill a row's last tile hold zeros.
+ *  row_scale  FP32 [n], NVFP4 only.
+ * Its value at (i, c) is e2m1 * scale(i, c / block) * row_scale[i]. codes and
+ * scales are 16-byte aligned, ldc is a multiple of 16. Tables made elsewhere in
+ * this layout can be multiplied as well (padding codes and scales zero). */
+int gat_b200_fp4_ld(int width);
+uint64_t gat_b200_fp4_scale_bytes(int format, uint64_t n, int width);
+
+/* x (FP32 or BF16, [n][ldx]) to a 4-bit table, every rounding to nearest even:
+ *  MXFP4: scale = 2^(floor(log2 amax) - 2), exponent at least -127;
+ *         code = e2m1(x / scale), saturating at 6.
+ *  NVFP4: row_scale = the smallest power of two r >= 2^-100 with
+ *         amax_row <= 2688 r (1 for a row of zeros); scale = e4m3(amax / (6 r));
+ *         code = e2m1(x / (scale r)); zeros where the scale is zero.
+ * amax: the largest magnitude of the block (amax_row: of the row). The codes
+ * are those of the exact quotients. A block (MXFP4) or row (NVFP4) with an Inf
+ * or NaN gets a NaN scale: all of it reads as NaN. If values is not NULL, what
+ * the table stands for is written there (FP32 or BF16, [n][ldv]; exact in
+ * both, but for magnitudes below the type's normal range). Scale bytes of rows
+ * past n are left as they were. */
+int gat_b200_fp4_quantize(int format, uint64_t n, int width, const void* x, int x_dtype, int ldx,
+                          void* codes, int ldc, void* scales, float* row_scale, void* values,
+                          int v_dtype, int ldv, void* stream);
+
+/* out[i][j] = sum_c a[i][c] b[j][c] over k columns of two tables of one format
+ * (a: m rows, for instance features; b: n rows, for instance the transposed
+ * weights), FP32 accumulation on the 4-bit tensor cores, times a_row[i] and
+ * b_row[j] (FP32, NULL = 1), rounded to out_dtype (FP32 or BF16), [m][ldo].
+ * lda / ldb: bytes per code row. Columns of out behind n are left as they
+ * were. */
+int gat_b200_fp4_product(int format, uint64_t m, int n, int k, const void* a, int lda,
+                         const void* a_scales, const float* a_row, const void* b, int ldb,
+                         const void* b_scales, const float* b_row, void* out, int out_dtype, int ldo,
+                         void* stream);
 
 /* m[i][h] = leaky(L_ih + max_{j in N(i)} R_jh), 0 for empty rows.
  * Replaces gat::max_prescan (baseline/src/baseline_standard.cpp:44-51). */
