@@ -1,0 +1,594 @@
+// Masked softmax attention inside the segments of a packed batch (tcgen05/TMA).
+//
+//   z_ij = cap tanh(scale q_i.k_j / cap) - slope_h |pos_i - pos_j|
+//   out_i = sum_j softmax_j(z_ij) v_j,   lse_i = log sum_j exp z_ij
+// over the keys j of row i's segment that its mask shows. Every mask here
+// (segment, causal, prefix) shows a row one interval [lo, hi) of packed keys,
+// so a tile of 128 packed rows may span many segments: small graphs share tiles
+// and a long document is one run of tiles.
+//
+// One CTA: two tiles of 128 rows of one head, all key blocks of 128 that one of
+// their rows sees. 12 warps:
+//   warp 0     TMA producer: Q once, K and V blocks through rings.
+//   warp 1     MMA issuer: S = Q K^T into TMEM; O += P V with P read from TMEM
+//              (P overlays S). The tiles alternate, so one tile's softmax runs
+//              beside the other's MMAs.
+//   warps 2-3  masked blocks only: take non-finite values of V out of shared
+//              memory (a weight of zero times Inf or NaN is NaN) and note their
+//              keys; rows that do see such a key add it themselves.
+//   warps 4-7 / 8-11  softmax of tile 0 / 1, a row per thread: no shuffles.
+// The running maximum is only moved when it grows by more than 8 (a factor of
+// 256 in the weights, far inside FP32 and BF16's range), so O is seldom rescaled.
+// MMAs of a CTA run in order, so S's barrier also says that the tile's last P V
+// is done and O is at rest. P is rounded to BF16 (the tensor cores' input type;
+// the sum keeps the unrounded FP32 weights).
+#include <cuda.h>
+
+#include "attention.cuh"
+#include "tc.cuh"
+
+namespace gatb {
+
+__device__ unsigned g_attention_error = 0;
+
+int make_tiled_map(CUtensorMap* m, int type, int rank, const void* base, const uint64_t* dims, const uint64_t* strides,
+                   const uint32_t* box, bool swizzle);
+
+namespace {
+
+using namespace tc;
+
+constexpr int kRows = 128;  // rows of a tile, keys of a block
+constexpr int kThreads = 384;
+
+struct AttnArgs {
+    uint64_t n_q, n_k;
+    int heads, group, dim, nseg, mask;
+    const uint64_t* q_row;
+    const uint64_t* k_row;
+    const uint64_t* prefix;
+    const float* slopes;
+    const uint16_t* v;
+    int ldv;
+    float zscale;    // without a cap: scale * log2 e; with one: 2 log2 e * scale / cap
+    float zcap;      // cap * log2 e
+    uint16_t* out;
+    int ldo;
+    float* lse;
+};
+
+// TMEM: S / P of tile t at 128 t, O of tile t at 256 + 128 t.
+__device__ __forceinline__ void mma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc) {
+    asm volatile("tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, 1;" ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc),
+                 "r"(idesc)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+// Largest s with row[s] <= i, of nseg + 1 ascending row pointers.
+__device__ __forceinline__ int segment_of(const uint64_t* row, int nseg, uint64_t i) {
+    int a = 0, b = nseg;
+    while (b - a > 1) {
+        const int mid = (a + b) >> 1;
+        if (row[mid] <= i)
+            a = mid;
+        else
+            b = mid;
+    }
+    return a;
+}
+
+// DP: dim rounded up to 64 or 128. CAP / BIAS: scores go through the tanh / get the distance bias.
+template <int DP, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnArgs g) {
+    constexpr int kTile = kRows * DP * 2;  // bytes of a Q tile, a K block, a V block
+    constexpr int kSt = DP == 64 ? 4 : 2;  // K and V stages
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* q_s = smem;
+    uint8_t* k_s = q_s + 2 * kTile;
+    uint8_t* v_s = k_s + kSt * kTile;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + kSt * kTile);
+    uint64_t* q_full = bars;
+    uint64_t* k_full = bars + 1;
+    uint64_t* k_empty = k_full + kSt;
+    uint64_t* v_full = k_empty + kSt;
+    uint64_t* v_ready = v_full + kSt;
+    uint64_t* v_empty = v_ready + kSt;
+    uint64_t* s_full = v_empty + kSt;  // [2]
+    uint64_t* p_full = s_full + 2;     // [2]
+    uint64_t* o_full = p_full + 2;     // [2]
+    uint32_t* bad = reinterpret_cast<uint32_t*>(o_full + 2);  // [kSt][4] keys of the block with non-finite values
+    unsigned* range = bad + 4 * kSt;  // per tile: smallest lo, largest hi, largest lo, smallest hi
+    uint32_t* tmem_holder = range + 8;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int head = blockIdx.y, kv_head = head / g.group;
+    // later rows see more keys under a causal mask: the longest tiles start first
+    const uint64_t row0 = uint64_t(gridDim.x - 1 - blockIdx.x) * (2 * kRows);
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        for (int s = 0; s < kSt; ++s) {
+            mbar_init(k_full + s, 1);
+            mbar_init(k_empty + s, 1);
+            mbar_init(v_full + s, 1);
+            mbar_init(v_ready + s, 2);
+            mbar_init(v_empty + s, 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(s_full + t, 1);
+            mbar_init(p_full + t, 4);
+            mbar_init(o_full + t, 1);
+            range[4 * t] = 0xffffffffu;
+            range[4 * t + 1] = 0;
+            range[4 * t + 2] = 0;
+            range[4 * t + 3] = 0xffffffffu;
+        }
+        *abort_flag = 0;
+        fence_mbarrier_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                     "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_holder;
+
+    // The row's key interval (softmax threads), its position and the tile's ranges.
+    const int tile = warp >= 8 ? 1 : 0;
+    const int r = (warp & 3) * 32 + lane;
+    const uint64_t row = row0 + uint64_t(tile) * kRows + r;
+    int lo = 0, hi = 0, pos = 0;
+    if (warp >= 4) {
+        const bool live = row < g.n_q;
+        if (live) {
+            const int s = segment_of(g.q_row, g.nseg, row);
+            // row pointers are taken as given but kept inside the tables
+            const uint64_t ks = min(g.k_row[s], g.n_k), ke = max(ks, min(g.k_row[s + 1], g.n_k));
+            const int64_t at = int64_t(row - min(g.q_row[s], row)) + int64_t(ke - ks) -
+                               int64_t(max(g.q_row[s + 1], g.q_row[s]) - g.q_row[s]);
+            lo = int(ks);
+            hi = int(ke);
+            if (g.mask != GAT_B200_MASK_FULL) {
+                int64_t seen = at + 1;
+                if (g.mask == GAT_B200_MASK_PREFIX) seen = max(seen, int64_t(min(g.prefix[s], g.n_k)));
+                seen = max(int64_t(0), min(seen, int64_t(ke - ks)));
+                hi = lo + int(seen);
+            }
+            pos = int(max(int64_t(-INT32_MAX), min(at, int64_t(INT32_MAX))));
+        }
+        const bool some = hi > lo;
+        const unsigned min_lo = __reduce_min_sync(0xffffffffu, some ? unsigned(lo) : 0xffffffffu);
+        const unsigned max_hi = __reduce_max_sync(0xffffffffu, some ? unsigned(hi) : 0u);
+        const unsigned max_lo = __reduce_max_sync(0xffffffffu, some ? unsigned(lo) : 0u);
+        const unsigned min_hi = __reduce_min_sync(0xffffffffu, some ? unsigned(hi) : 0xffffffffu);
+        if (lane == 0) {
+            atomicMin(range + 4 * tile, min_lo);
+            atomicMax(range + 4 * tile + 1, max_hi);
+            atomicMax(range + 4 * tile + 2, max_lo);
+            atomicMin(range + 4 * tile + 3, min_hi);
+        }
+    }
+    __syncthreads();
+    const unsigned first_key = min(range[0], range[4]), end_key = max(range[1], range[5]);
+    const int blocks = end_key > first_key ? int((end_key - first_key + kRows - 1) / kRows) : 0;
+    // key blocks [from, to) that tile t works on
+    int from[2], to[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const bool any = range[4 * t + 1] > range[4 * t];
+        from[t] = any ? int((range[4 * t] - first_key) / kRows) : 0;
+        to[t] = any ? int((range[4 * t + 1] - first_key + kRows - 1) / kRows) : 0;
+    }
+    const int last_tile = to[1] > 0 ? 1 : 0;
+    // blocks [clean_from, clean_to) are seen whole by every row that sees anything
+    const unsigned max_lo = max(range[2], range[6]), min_hi = min(range[3], range[7]);
+    const int ksteps = (g.dim + 15) / 16;
+
+    if (blocks == 0) {
+        // nothing to see: zeros below
+    } else if (warp == 0) {
+        if (lane == 0) {
+            const int boxes = g.dim > 64 ? 2 : 1;
+            const uint32_t bytes = uint32_t(boxes) * kRows * 128;
+            mbar_expect_tx(q_full, bytes * (last_tile + 1));
+            for (int t = 0; t <= last_tile; ++t)
+                for (int b = 0; b < boxes; ++b)
+                    tma_load_3d(q_s + t * kTile + b * (kRows * 128), &tm_q, q_full, b * 64, head, int(row0) + t * kRows);
+            bool ok = true;
+            int j = 0;
+            for (; j < blocks && ok; ++j) {
+                const int s = j % kSt;
+                const uint32_t ph = uint32_t(j / kSt) & 1u;
+                const int key = int(first_key) + j * kRows;
+                if (!mbar_wait(k_empty + s, ph ^ 1u, abort_flag, &g_attention_error)) { ok = false; break; }
+                mbar_expect_tx(k_full + s, bytes);
+                for (int b = 0; b < boxes; ++b)
+                    tma_load_3d(k_s + s * kTile + b * (kRows * 128), &tm_k, k_full + s, b * 64, kv_head, key);
+                if (!mbar_wait(v_empty + s, ph ^ 1u, abort_flag, &g_attention_error)) {
+                    mbar_wait(k_full + s, ph, abort_flag, &g_attention_error);
+                    ok = false;
+                    break;
+                }
+                mbar_expect_tx(v_full + s, bytes);
+                for (int b = 0; b < boxes; ++b)
+                    tma_load_3d(v_s + s * kTile + b * (kRows * 128), &tm_v, v_full + s, b * 64, kv_head, key);
+            }
+            // the loads still in flight land before the CTA ends
+            mbar_wait(q_full, 0, abort_flag, &g_attention_error);
+            for (int i = j > kSt ? j - kSt : 0; i < j; ++i) {
+                mbar_wait(k_full + i % kSt, uint32_t(i / kSt) & 1u, abort_flag, &g_attention_error);
+                mbar_wait(v_full + i % kSt, uint32_t(i / kSt) & 1u, abort_flag, &g_attention_error);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc_s = idesc_bf16(kRows, kRows, 0, 0);
+            const uint32_t idesc_o = idesc_bf16(kRows, ksteps * 16, 0, 1);
+            bool ok = mbar_wait(q_full, 0, abort_flag, &g_attention_error);
+            uint32_t used[2] = {0, 0};  // blocks of tile t issued so far
+            auto scores = [&](int t, int j) {
+                const uint32_t qa = smem_u32(q_s + t * kTile), ka = smem_u32(k_s + (j % kSt) * kTile);
+                for (int ks = 0; ks < ksteps; ++ks) {
+                    const uint32_t off = (ks >> 2) * (kRows * 128) + (ks & 3) * 32;
+                    mma_bf16(tmem + 128 * t, desc_sw128(qa + off, 16, 1024), desc_sw128(ka + off, 16, 1024), idesc_s, ks > 0);
+                }
+                mma_commit(s_full + t);
+            };
+            for (int j = -1; j < blocks && ok; ++j) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (t > last_tile || !ok) break;
+                    if (j >= 0) {
+                        const int s = j % kSt;
+                        if (t == 0 && !mbar_wait(v_ready + s, uint32_t(j / kSt) & 1u, abort_flag, &g_attention_error)) { ok = false; break; }
+                        if (j >= from[t] && j < to[t]) {
+                            if (!mbar_wait(p_full + t, used[t] & 1u, abort_flag, &g_attention_error)) { ok = false; break; }
+                            ++used[t];
+                            fence_after();
+                            const uint32_t va = smem_u32(v_s + s * kTile);
+#pragma unroll
+                            for (int ks = 0; ks < kRows / 16; ++ks)
+                                mma_bf16_ts(tmem + 256 + 128 * t, tmem + 128 * t + ks * 8,
+                                            desc_sw128(va + ks * 2048, kRows * 128, 1024), idesc_o);
+                            if (j + 1 == to[t]) mma_commit(o_full + t);
+                        }
+                        if (t == last_tile) mma_commit(v_empty + s);
+                    }
+                    if (j + 1 < blocks) {
+                        const int s = (j + 1) % kSt;
+                        if (t == 0 && !mbar_wait(k_full + s, uint32_t((j + 1) / kSt) & 1u, abort_flag, &g_attention_error)) { ok = false; break; }
+                        if (j + 1 >= from[t] && j + 1 < to[t]) {
+                            fence_after();
+                            scores(t, j + 1);
+                        }
+                        if (t == last_tile) mma_commit(k_empty + s);
+                    }
+                }
+            }
+            // whatever was issued has finished before the CTA ends (v_empty of the last block)
+            if (ok)
+                mbar_wait(v_empty + (blocks - 1) % kSt, uint32_t((blocks - 1) / kSt) & 1u, abort_flag, &g_attention_error);
+        }
+    } else if (warp < 4) {
+        // ---- V of masked blocks: non-finite values out, their keys noted ----
+        for (int j = 0; j < blocks; ++j) {
+            const int s = j % kSt;
+            if (!mbar_wait(v_full + s, uint32_t(j / kSt) & 1u, abort_flag, &g_attention_error)) break;
+            const unsigned key = first_key + unsigned(j) * kRows;
+            if (key < max_lo || key + kRows > min_hi) {
+                uint32_t* words = bad + 4 * s;
+                const int half = warp - 2;  // 64 keys a warp
+                if (lane < 2) words[2 * half + lane] = 0;
+                __syncwarp();
+                const int boxes = g.dim > 64 ? 2 : 1;
+                for (int b = 0; b < boxes; ++b) {
+                    uint8_t* base = v_s + s * kTile + b * (kRows * 128) + half * 64 * 128;
+#pragma unroll 4
+                    for (int i = lane; i < 64 * 8; i += 32) {
+                        uint4 w = *reinterpret_cast<const uint4*>(base + i * 16);
+                        auto hit = [](uint32_t x) {
+                            return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+                        };
+                        if (hit(w.x) | hit(w.y) | hit(w.z) | hit(w.w)) {
+                            auto clean = [](uint32_t x) {
+                                if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
+                                if ((x & 0x7f800000u) == 0x7f800000u) x &= 0xffffu;
+                                return x;
+                            };
+                            *reinterpret_cast<uint4*>(base + i * 16) =
+                                make_uint4(clean(w.x), clean(w.y), clean(w.z), clean(w.w));
+                            const int k = half * 64 + (i >> 3);
+                            atomicOr(words + (k >> 5), 1u << (k & 31));
+                        }
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+            }
+            if (lane == 0) mbar_arrive(v_ready + s);
+        }
+    } else if (to[tile] > 0) {
+        // ---- softmax of one tile: thread = row ----
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        const uint32_t s_t = tmem + lanes + 128 * tile, o_t = tmem + lanes + 256 + 128 * tile;
+        const float nslope = BIAS ? -g.slopes[head] * kLog2e : 0.f;
+        {
+            uint32_t z[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[i] = 0;
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) tmem_st32(o_t + c, z);
+            tmem_wait_st();
+        }
+        float m = -INFINITY, l = 0.f;  // reference maximum (log2 units) and sum of weights
+        bool ok = true;
+        uint32_t use = 0;
+        for (int j = from[tile]; j < to[tile]; ++j, ++use) {
+            if (!mbar_wait(s_full + tile, use & 1u, abort_flag, &g_attention_error)) { ok = false; break; }
+            fence_after();
+            const int key = int(first_key) + j * kRows;
+            const int jl = lo - key, jh = hi - key;  // visible columns [jl, jh)
+            const bool whole = __all_sync(0xffffffffu, (jl <= 0 && jh >= kRows) || hi <= lo);
+            float z[kRows];
+            tmem_ld64(s_t, z);
+            tmem_ld64(s_t + 64, z + 64);
+            if constexpr (CAP) {
+#pragma unroll
+                for (int c = 0; c < kRows; ++c) z[c] = g.zcap * tanh_of_log2(z[c] * g.zscale);
+            }
+            if constexpr (BIAS) {
+                const float rel = float(pos + jl);
+#pragma unroll
+                for (int c = 0; c < kRows; ++c) {
+                    if constexpr (!CAP) z[c] *= g.zscale;
+                    z[c] = fmaf(nslope, fabsf(rel - float(c)), z[c]);
+                }
+            }
+            if (!whole) {
+#pragma unroll
+                for (int c = 0; c < kRows; ++c) z[c] = c >= jl && c < jh ? z[c] : -INFINITY;
+            }
+            float mb = z[0];
+#pragma unroll
+            for (int c = 1; c < kRows; ++c) mb = fmaxf(mb, z[c]);
+            if constexpr (!CAP && !BIAS) mb *= g.zscale;
+            if (m == -INFINITY) m = mb;
+            const bool grow = mb > m + 8.f;
+            if (__any_sync(0xffffffffu, grow)) {
+                const float f = grow ? ex2(m - mb) : 1.f;
+                if (grow) m = mb;
+                l *= f;
+#pragma unroll
+                for (int c = 0; c < DP; c += 32) {
+                    float o[32];
+                    tmem_ld32(o_t + c, o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] *= f;
+                    tmem_st32(o_t + c, reinterpret_cast<const uint32_t*>(o));
+                }
+                tmem_wait_st();
+            }
+            const float ref = m == -INFINITY ? 0.f : m;
+            uint32_t p[kRows / 2];
+            float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+            for (int c = 0; c < kRows; c += 2) {
+                float p0, p1;
+                if constexpr (CAP || BIAS) {
+                    p0 = ex2(z[c] - ref);
+                    p1 = ex2(z[c + 1] - ref);
+                } else {
+                    p0 = ex2(fmaf(z[c], g.zscale, -ref));
+                    p1 = ex2(fmaf(z[c + 1], g.zscale, -ref));
+                }
+                sum0 += p0;
+                sum1 += p1;
+                p[c / 2] = pack_bf16x2(p0, p1);
+            }
+            l += sum0 + sum1;
+            tmem_st32(s_t, p);
+            tmem_st32(s_t + 32, p + 32);
+            if (unsigned(key) < max_lo || unsigned(key) + kRows > min_hi) {
+                // keys with non-finite values that this row sees: their weights times those values
+                const int s = j % kSt;
+                if (!mbar_wait(v_ready + s, uint32_t(j / kSt) & 1u, abort_flag, &g_attention_error)) { ok = false; break; }
+#pragma unroll 1
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t bits = bad[4 * s + w];
+                    while (bits) {  // the same for the whole warp
+                        const int c = w * 32 + __ffs(bits) - 1;
+                        bits &= bits - 1;
+                        uint32_t pw = 0;
+#pragma unroll
+                        for (int i = 0; i < kRows / 2; ++i)
+                            if (i == c / 2) pw = p[i];
+                        const float pc = (c & 1) ? bf16hi(pw) : bf16lo(pw);
+                        const bool mine = c >= jl && c < jh;
+                        const uint16_t* vr = g.v + (uint64_t(key) + c) * uint64_t(g.ldv) + uint64_t(kv_head) * g.dim;
+#pragma unroll 1
+                        for (int x = 0; x < DP; x += 8) {
+                            float o[8];
+                            tmem_ld8(o_t + x, o);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if (mine && x + i < g.dim) {
+                                    const uint32_t e = vr[x + i];
+                                    if ((e & 0x7f80u) == 0x7f80u) o[i] += pc * bf16lo(e);
+                                }
+                            const uint32_t* ou = reinterpret_cast<const uint32_t*>(o);
+                            asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(
+                                             o_t + x),
+                                         "r"(ou[0]), "r"(ou[1]), "r"(ou[2]), "r"(ou[3]), "r"(ou[4]), "r"(ou[5]),
+                                         "r"(ou[6]), "r"(ou[7])
+                                         : "memory");
+                        }
+                    }
+                }
+            }
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + tile);
+        }
+        if (ok && mbar_wait(o_full + tile, 0, abort_flag, &g_attention_error)) {
+            fence_after();
+            const float inv = hi > lo ? 1.f / l : 0.f;
+            const bool live = row < g.n_q;
+            uint16_t* orow = g.out + row * uint64_t(g.ldo) + uint64_t(head) * g.dim;
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 32) {
+                float o[32];
+                tmem_ld32(o_t + c, o);
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        if (c + i >= g.dim) break;
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = hi > lo ? pack_bf16x2(o[i + 2 * e] * inv, o[i + 2 * e + 1] * inv) : 0u;
+                        *reinterpret_cast<uint4*>(orow + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                __syncwarp();
+            }
+            if (live && g.lse) g.lse[row * g.heads + head] = hi > lo ? (m + log2f(l)) * kLn2 : -INFINITY;
+        }
+    }
+    // tiles whose rows all see nothing
+    if (warp >= 4 && to[tile] == 0 && row < g.n_q) {
+        uint16_t* orow = g.out + row * uint64_t(g.ldo) + uint64_t(head) * g.dim;
+        for (int c = 0; c < g.dim; c += 8) *reinterpret_cast<uint4*>(orow + c) = make_uint4(0, 0, 0, 0);
+        if (g.lse) g.lse[row * g.heads + head] = -INFINITY;
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+int heads_map(CUtensorMap* m, const void* base, int dim, int heads, uint64_t rows, int ld) {
+    const uint64_t dims[3] = {uint64_t(dim), uint64_t(heads), rows};
+    const uint64_t strides[2] = {uint64_t(dim) * 2, uint64_t(ld) * 2};
+    const uint32_t box[3] = {64, 1, kRows};
+    return make_tiled_map(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box, true);
+}
+
+template <int DP, bool CAP, bool BIAS>
+int launch(const AttnArgs& g, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
+    constexpr int kSt = DP == 64 ? 4 : 2;
+    constexpr int smem = (2 + 2 * kSt) * kRows * DP * 2 + 1024 + 512;
+    auto kern = attention_kernel<DP, CAP, BIAS>;
+    GATB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    const dim3 grid(unsigned((g.n_q + 2 * kRows - 1) / (2 * kRows)), unsigned(g.heads));
+    kern<<<grid, kThreads, smem, st>>>(q, k, v, g);
+    GATB_LAUNCH("masked_attention kernel");
+    return 0;
+}
+template <int DP>
+int launch(const AttnArgs& g, bool cap, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+           cudaStream_t st) {
+    if (cap) return g.slopes ? launch<DP, true, true>(g, q, k, v, st) : launch<DP, true, false>(g, q, k, v, st);
+    return g.slopes ? launch<DP, false, true>(g, q, k, v, st) : launch<DP, false, false>(g, q, k, v, st);
+}
+
+}  // namespace
+
+int attention_check(const char* what, const AttentionShape& s, uint64_t n_q, uint64_t n_k, int nseg, const void* q,
+                    int ldq, const void* k, int ldk, const void* v, int ldv, const void* out, int ldo) {
+    const std::string w = std::string(what) + ": ";
+    if (s.heads <= 0 || s.heads > 65535 || s.kv_heads <= 0 || s.heads % s.kv_heads)
+        return fail(w + "heads must be a multiple of kv_heads");
+    if (s.dim <= 0 || s.dim > 128 || s.dim % 8) return fail_code(GAT_B200_EUNSUPPORTED, w + "dim must be a multiple of 8, at most 128");
+    if (n_q > uint64_t(INT32_MAX - 512) || n_k > uint64_t(INT32_MAX - 512)) return fail(w + "too many rows");
+    if (nseg < 0) return fail(w + "bad segment count");
+    if (!(s.scale > 0.f) || !(s.scale < 3e38f)) return fail(w + "scale must be positive and finite");
+    if (!(s.cap >= 0.f) || !(s.cap < 3e38f)) return fail(w + "cap must be finite and not negative (0: none)");
+    const int64_t hq = int64_t(s.heads) * s.dim, hk = int64_t(s.kv_heads) * s.dim;
+    if (ldq < hq || ldk < hk || ldv < hk || ldo < hq) return fail(w + "row stride smaller than heads * dim");
+    if ((ldq | ldk | ldv | ldo) % 8) return fail(w + "rows must be 16-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+         reinterpret_cast<uintptr_t>(out)) & 15)
+        return fail(w + "rows must be 16-byte aligned");
+    return 0;
+}
+
+int masked_attention_launch(const AttentionShape& s, int nseg, uint64_t n_q, uint64_t n_k, const uint64_t* q_row,
+                            const uint64_t* k_row, int mask, const uint64_t* prefix, const void* q, int ldq,
+                            const void* k, int ldk, const void* v, int ldv, void* out, int ldo, float* lse,
+                            cudaStream_t st) {
+    if (int rc = attention_check("masked_attention", s, n_q, n_k, nseg, q, ldq, k, ldk, v, ldv, out, ldo)) return rc;
+    if (mask < GAT_B200_MASK_FULL || mask > GAT_B200_MASK_PREFIX) return fail("masked_attention: bad mask");
+    if (mask == GAT_B200_MASK_PREFIX && !prefix) return fail("masked_attention: the prefix mask needs the prefix lengths");
+    if (n_q == 0) return 0;
+    if (nseg == 0) return fail("masked_attention: rows without segments");
+    if (!q_row || !k_row || !q || !out || (n_k && (!k || !v))) return fail("masked_attention: null argument");
+    if ((reinterpret_cast<uintptr_t>(q_row) | reinterpret_cast<uintptr_t>(k_row) | reinterpret_cast<uintptr_t>(prefix)) % 8 ||
+        (reinterpret_cast<uintptr_t>(s.slopes) | reinterpret_cast<uintptr_t>(lse)) % 4)
+        return fail("masked_attention: misaligned pointer");
+    if (int rc = check_device_pointers("masked_attention", {q_row, k_row, prefix, q, k, v, s.slopes, out, lse})) return rc;
+    AttnArgs g{};
+    g.n_q = n_q;
+    g.n_k = n_k;
+    g.heads = s.heads;
+    g.group = s.heads / s.kv_heads;
+    g.dim = s.dim;
+    g.nseg = nseg;
+    g.mask = mask;
+    g.q_row = q_row;
+    g.k_row = k_row;
+    g.prefix = mask == GAT_B200_MASK_PREFIX ? prefix : nullptr;
+    g.slopes = s.slopes;
+    g.v = static_cast<const uint16_t*>(v);
+    g.ldv = ldv;
+    g.zscale = s.cap > 0.f ? 2.f * kLog2e * s.scale / s.cap : s.scale * kLog2e;
+    g.zcap = s.cap * kLog2e;
+    g.out = static_cast<uint16_t*>(out);
+    g.ldo = ldo;
+    g.lse = lse;
+    CUtensorMap tq, tk, tv;
+    if (int rc = heads_map(&tq, q, s.dim, s.heads, n_q, ldq)) return rc;
+    // without keys nothing is loaded: any valid map will do
+    if (int rc = heads_map(&tk, n_k ? k : q, s.dim, n_k ? s.kv_heads : s.heads, n_k ? n_k : n_q, n_k ? ldk : ldq)) return rc;
+    if (int rc = heads_map(&tv, n_k ? v : q, s.dim, n_k ? s.kv_heads : s.heads, n_k ? n_k : n_q, n_k ? ldv : ldq)) return rc;
+    return s.dim <= 64 ? launch<64>(g, s.cap > 0.f, tq, tk, tv, st) : launch<128>(g, s.cap > 0.f, tq, tk, tv, st);
+}
+
+int attention_check_error() {
+    unsigned e = 0;
+    GATB_CUDA(cudaMemcpyFromSymbol(&e, g_attention_error, sizeof(e)));
+    if (e) {
+        unsigned z = 0;
+        cudaMemcpyToSymbol(g_attention_error, &z, sizeof(z));
+        return fail_code(GAT_B200_ETIMEOUT, "masked_attention kernel: a bounded wait timed out");
+    }
+    return 0;
+}
+
+}  // namespace gatb

@@ -8,6 +8,7 @@
 
 #include <nvtx3/nvToolsExt.h>
 
+#include "attention.cuh"
 #include "device.cuh"
 #include "graph.cuh"
 
@@ -43,13 +44,24 @@ int fp4_product_launch(int format, uint64_t m, int n, int k, const void* a, int 
                        const float* a_row, const void* b, int ldb, const void* b_scales, const float* b_row, void* out,
                        int out_dtype, int ldo, cudaStream_t st);
 int fp4_check_error();
+int masked_attention_launch(const AttentionShape& s, int nseg, uint64_t n_q, uint64_t n_k, const uint64_t* q_row,
+                            const uint64_t* k_row, int mask, const uint64_t* prefix, const void* q, int ldq,
+                            const void* k, int ldk, const void* v, int ldv, void* out, int ldo, float* lse,
+                            cudaStream_t st);
+uint64_t masked_attention_step_workspace(int heads, int dim, int nseg);
+int masked_attention_step_launch(const AttentionShape& s, int nseg, uint64_t n_k, const uint64_t* begin,
+                                 const uint64_t* length, const void* q, int ldq, const void* k, int ldk, const void* v,
+                                 int ldv, void* out, int ldo, float* lse, void* workspace, uint64_t workspace_bytes,
+                                 cudaStream_t st);
+int attention_check_error();
 int device_check_errors() {
     int rc = projection_tc_check_error();
     int rc2 = aggregate_check_error();
     int rc3 = tfs_tc_check_error();
     int rc4 = peer_check_error();
     int rc5 = fp4_check_error();
-    return rc ? rc : (rc2 ? rc2 : (rc3 ? rc3 : (rc4 ? rc4 : rc5)));
+    int rc6 = attention_check_error();
+    return rc ? rc : (rc2 ? rc2 : (rc3 ? rc3 : (rc4 ? rc4 : (rc5 ? rc5 : rc6))));
 }
 
 namespace {
@@ -368,6 +380,28 @@ int gat_b200_fp4_product(int format, uint64_t m, int n, int k, const void* a, in
     clear_error();
     return fp4_product_launch(format, m, n, k, a, lda, a_scales, a_row, b, ldb, b_scales, b_row, out, out_dtype, ldo,
                               as_stream(stream));
+}
+
+int gat_b200_masked_attention(int heads, int kv_heads, int dim, int nseg, uint64_t n_q, uint64_t n_k,
+                              const uint64_t* q_row, const uint64_t* k_row, int mask, const uint64_t* prefix,
+                              const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, float scale,
+                              float cap, const float* slopes, void* out, int ldo, float* lse, void* stream) {
+    clear_error();
+    return masked_attention_launch({heads, kv_heads, dim, scale, cap, slopes}, nseg, n_q, n_k, q_row, k_row, mask,
+                                   prefix, q, ldq, k, ldk, v, ldv, out, ldo, lse, as_stream(stream));
+}
+
+uint64_t gat_b200_masked_attention_step_workspace(int heads, int dim, int nseg) {
+    return masked_attention_step_workspace(heads, dim, nseg);
+}
+
+int gat_b200_masked_attention_step(int heads, int kv_heads, int dim, int nseg, uint64_t n_k, const uint64_t* begin,
+                                   const uint64_t* length, const void* q, int ldq, const void* k, int ldk,
+                                   const void* v, int ldv, float scale, float cap, const float* slopes, void* out,
+                                   int ldo, float* lse, void* workspace, uint64_t workspace_bytes, void* stream) {
+    clear_error();
+    return masked_attention_step_launch({heads, kv_heads, dim, scale, cap, slopes}, nseg, n_k, begin, length, q, ldq, k,
+                                        ldk, v, ldv, out, ldo, lse, workspace, workspace_bytes, as_stream(stream));
 }
 
 int gat_b200_projection_scatter(const gat_b200_layer* p, uint64_t n, const void* x, int ldx, void* h, int ldh,

@@ -30,6 +30,7 @@ _lib = C.CDLL(str(LIB_PATH))
 
 F32, BF16 = 0, 1
 MXFP4, NVFP4 = 2, 3
+MASK_FULL, MASK_CAUSAL, MASK_PREFIX = 0, 1, 2
 PATH_STANDARD_BF16, PATH_STANDARD_FP32, PATH_TFS_BF16, PATH_ADAPTIVE_BF16, PATH_MATCHED_ATTENTION = 0, 1, 2, 3, 4
 TFS_EDGE, TFS_BLOCK, TFS_SPLIT = 0, 1, 2
 LR_BF16, LR_FP32 = 0, 1
@@ -85,6 +86,13 @@ SIGNATURES = [
                                         _vp, C.c_int, C.c_int, _vp]),
     ("gat_b200_fp4_product", C.c_int, [C.c_int, C.c_uint64, C.c_int, C.c_int, _vp, C.c_int, _vp, _vp, _vp, C.c_int,
                                        _vp, _vp, _vp, C.c_int, C.c_int, _vp]),
+    ("gat_b200_masked_attention", C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_uint64, C.c_uint64, _vp, _vp, C.c_int,
+                                            _vp, _vp, C.c_int, _vp, C.c_int, _vp, C.c_int, C.c_float, C.c_float, _vp, _vp,
+                                            C.c_int, _vp, _vp]),
+    ("gat_b200_masked_attention_step_workspace", C.c_uint64, [C.c_int, C.c_int, C.c_int]),
+    ("gat_b200_masked_attention_step", C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_uint64, _vp, _vp, _vp, C.c_int,
+                                                 _vp, C.c_int, _vp, C.c_int, C.c_float, C.c_float, _vp, _vp, C.c_int,
+                                                 _vp, _vp, C.c_uint64, _vp]),
     ("gat_b200_max_prescan", C.c_int, [_vp, C.c_int, _vp, _vp, _vp, _vp]),
     ("gat_b200_edge_softmax", C.c_int, [_vp, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     ("gat_b200_standard_aggregate", C.c_int, [_vp, C.c_int, C.c_int, _vp, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp, C.c_int, _vp, _vp, _vp]),
@@ -494,6 +502,27 @@ def fp4_product(fmt: int, m, n, k, a, lda, a_scales, a_row, b, ldb, b_scales, b_
     """out = a b^T of two 4-bit tables (gat_b200_fp4_product)."""
     _check(_lib.gat_b200_fp4_product(fmt, m, n, k, _ptr(a), lda, _ptr(a_scales), _ptr(a_row), _ptr(b), ldb,
                                      _ptr(b_scales), _ptr(b_row), _ptr(out), out_dtype, ldo, _stream(stream)))
+
+
+def masked_attention(heads, kv_heads, dim, nseg, n_q, n_k, q_row, k_row, mask, prefix, q, ldq, k, ldk, v, ldv, scale,
+                     cap, slopes, out, ldo, lse=None, stream=None):
+    """Softmax attention inside the segments of a packed batch (gat_b200_masked_attention)."""
+    _check(_lib.gat_b200_masked_attention(heads, kv_heads, dim, nseg, n_q, n_k, _ptr(q_row), _ptr(k_row), mask,
+                                          _ptr(prefix), _ptr(q), ldq, _ptr(k), ldk, _ptr(v), ldv, scale, cap,
+                                          _ptr(slopes), _ptr(out), ldo, _ptr(lse), _stream(stream)))
+
+
+def masked_attention_step_workspace(heads: int, dim: int, nseg: int) -> int:
+    """Workspace bytes of masked_attention_step."""
+    return _lib.gat_b200_masked_attention_step_workspace(heads, dim, nseg)
+
+
+def masked_attention_step(heads, kv_heads, dim, nseg, n_k, begin, length, q, ldq, k, ldk, v, ldv, scale, cap, slopes,
+                          out, ldo, lse, workspace, workspace_bytes, stream=None):
+    """The same for one new row per segment over its keys (gat_b200_masked_attention_step)."""
+    _check(_lib.gat_b200_masked_attention_step(heads, kv_heads, dim, nseg, n_k, _ptr(begin), _ptr(length), _ptr(q), ldq,
+                                               _ptr(k), ldk, _ptr(v), ldv, scale, cap, _ptr(slopes), _ptr(out), ldo,
+                                               _ptr(lse), _ptr(workspace), workspace_bytes, _stream(stream)))
 
 
 PEER_HANDLE_BYTES = 64

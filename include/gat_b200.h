@@ -43,6 +43,12 @@ extern "C" {
 #define GAT_B200_MXFP4 2 /* E2M1, blocks of 32 columns, E8M0 scale */
 #define GAT_B200_NVFP4 3 /* E2M1, blocks of 16 columns, E4M3 scale, FP32 scale per row */
 
+/* Masks of gat_b200_masked_attention, inside a segment of lq rows and lk keys:
+ * row i stands at position i + lk - lq, so the last row sees the last key. */
+#define GAT_B200_MASK_FULL 0   /* every key of the segment */
+#define GAT_B200_MASK_CAUSAL 1 /* keys at or before the row's position */
+#define GAT_B200_MASK_PREFIX 2 /* as CAUSAL, and the segment's first prefix[s] keys */
+
 /* Layer paths, named after the reference's --path values
  * (baseline/bench/main.cpp:30, baseline/src/common.cpp:126-134). */
 #define GAT_B200_PATH_STANDARD_BF16 0 /* B0: BF16 X/W on tcgen05, FP32 softmax state */
@@ -338,6 +344,46 @@ int gat_b200_aggregate_fused_noalloc(uint64_t n, uint64_t e, const uint64_t* row
                                      const uint32_t* col, int heads, int dim, const void* h,
                                      int h_dtype, int ldh, const float* left, const float* right,
                                      int hidden, void* out, int out_dtype, int ldo, void* stream);
+
+/* ---- dense masked attention (no counterpart in the reference, whose
+ * attention runs over given edges) ----------------------------------------- */
+
+/* Softmax attention inside the segments (graphs, documents) of a packed batch,
+ * for row i of segment s and head h over the keys j that the mask shows:
+ *   z_ij  = cap * tanh(scale * q_i.k_j / cap)   (cap 0: scale * q_i.k_j)
+ *           - slopes[h] * |position of i - j|    (slopes NULL: no bias)
+ *   out_i = sum_j exp(z_ij) v_j / sum_j exp(z_ij),  lse_i = log sum_j exp(z_ij)
+ * Rows q_row[s] .. q_row[s+1] and keys k_row[s] .. k_row[s+1] (device, uint64
+ * [nseg+1], as a CSR's row pointers: q_row[0] = 0, q_row[nseg] = n_q,
+ * non-decreasing) belong to segment s; a segment may have no rows or no keys.
+ * Like the CSR of gat_b200_aggregate_fused_noalloc they are read as given, but
+ * kept inside n_q and n_k. prefix: device uint64 [nseg], MASK_PREFIX only.
+ * A row that sees no key gets zeros and lse -inf. What a row does not see never
+ * reaches it, Inf and NaN included.
+ * q, out: BF16 [n_q][heads * dim]; k, v: BF16 [n_k][kv_heads * dim]; query head
+ * h reads key head h / (heads / kv_heads). ld* are row strides in elements;
+ * rows 16-byte aligned. lse: FP32 [n_q][heads] or NULL. slopes: FP32 [heads].
+ * dim: a multiple of 8, at most 128 (GAT_B200_EUNSUPPORTED otherwise). Scores
+ * and sums are FP32; the weights are rounded to BF16 for the second product. */
+int gat_b200_masked_attention(int heads, int kv_heads, int dim, int nseg, uint64_t n_q, uint64_t n_k,
+                              const uint64_t* q_row, const uint64_t* k_row, int mask,
+                              const uint64_t* prefix, const void* q, int ldq, const void* k, int ldk,
+                              const void* v, int ldv, float scale, float cap, const float* slopes,
+                              void* out, int ldo, float* lse, void* stream);
+
+/* The same for one new row per segment, the last one of its segment (so it
+ * sees every key): q, out BF16 [nseg][heads * dim]; segment s has the keys
+ * begin[s] .. begin[s] + length[s] of the tables k and v of n_k rows (device,
+ * uint64 [nseg]; segments may overlap and leave gaps, what reaches past n_k is
+ * cut off). Lengths may change between replays of a captured call. workspace:
+ * device memory of at least gat_b200_masked_attention_step_workspace() bytes,
+ * 16-byte aligned, not shared with a call that may run at the same time. */
+uint64_t gat_b200_masked_attention_step_workspace(int heads, int dim, int nseg);
+int gat_b200_masked_attention_step(int heads, int kv_heads, int dim, int nseg, uint64_t n_k,
+                                   const uint64_t* begin, const uint64_t* length, const void* q,
+                                   int ldq, const void* k, int ldk, const void* v, int ldv, float scale,
+                                   float cap, const float* slopes, void* out, int ldo, float* lse,
+                                   void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* One full layer on device buffers. Replaces gat::standard_layer
  * (baseline/src/baseline_standard.cpp:98-108) for path STANDARD_BF16 (x BF16)
