@@ -122,9 +122,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t* tmem_holder = range + 8;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int head = blockIdx.y, kv_head = head / g.group;
-    // later rows see more keys under a causal mask: the longest tiles start first
-    const uint64_t row0 = uint64_t(gridDim.x - 1 - blockIdx.x) * (2 * kRows);
+    const int head = int(blockIdx.x % unsigned(g.heads)), kv_head = head / g.group;
+    // later rows see more keys under a causal mask: the longest tiles of all heads start first
+    const uint64_t row0 = uint64_t((gridDim.x - 1 - blockIdx.x) / unsigned(g.heads)) * (2 * kRows);
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
@@ -207,9 +207,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     // blocks [clean_from, clean_to) are seen whole by every row that sees anything
     const unsigned max_lo = max(range[2], range[6]), min_hi = min(range[3], range[7]);
     const int ksteps = (g.dim + 15) / 16;
-
+    // 384 threads start with 168 registers (64,512): 128 x 72 + 256 x 216 of them afterwards
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (blocks == 0) {
-        // nothing to see: zeros below
+        // nothing to see: the softmax warps write zeros
     } else if (warp == 0) {
         if (lane == 0) {
             const int boxes = g.dim > 64 ? 2 : 1;
@@ -331,7 +333,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (lane == 0) mbar_arrive(v_ready + s);
         }
-    } else if (to[tile] > 0) {
+    }
+    } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int my_from = tile ? from[1] : from[0], my_to = tile ? to[1] : to[0];
+    if (my_to > 0) {
         // ---- softmax of one tile: thread = row ----
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
         const uint32_t s_t = tmem + lanes + 128 * tile, o_t = tmem + lanes + 256 + 128 * tile;
@@ -347,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float m = -INFINITY, l = 0.f;  // reference maximum (log2 units) and sum of weights
         bool ok = true;
         uint32_t use = 0;
-        for (int j = from[tile]; j < to[tile]; ++j, ++use) {
+        for (int j = my_from; j < my_to; ++j, ++use) {
             if (!mbar_wait(s_full + tile, use & 1u, abort_flag, &g_attention_error)) { ok = false; break; }
             fence_after();
             const int key = int(first_key) + j * kRows;
@@ -416,16 +422,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // keys with non-finite values that this row sees: their weights times those values
                 const int s = j % kSt;
                 if (!mbar_wait(v_ready + s, uint32_t(j / kSt) & 1u, abort_flag, &g_attention_error)) { ok = false; break; }
+                tmem_wait_st();
 #pragma unroll 1
                 for (int w = 0; w < 4; ++w) {
                     uint32_t bits = bad[4 * s + w];
                     while (bits) {  // the same for the whole warp
                         const int c = w * 32 + __ffs(bits) - 1;
                         bits &= bits - 1;
-                        uint32_t pw = 0;
-#pragma unroll
-                        for (int i = 0; i < kRows / 2; ++i)
-                            if (i == c / 2) pw = p[i];
+                        uint32_t pw;
+                        asm volatile(
+                            "tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;"
+                            : "=r"(pw)
+                            : "r"(s_t + c / 2)
+                            : "memory");
                         const float pc = (c & 1) ? bf16hi(pw) : bf16lo(pw);
                         const bool mine = c >= jl && c < jh;
                         const uint16_t* vr = g.v + (uint64_t(key) + c) * uint64_t(g.ldv) + uint64_t(kv_head) * g.dim;
@@ -479,11 +488,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (live && g.lse) g.lse[row * g.heads + head] = hi > lo ? (m + log2f(l)) * kLn2 : -INFINITY;
         }
     }
-    // tiles whose rows all see nothing
-    if (warp >= 4 && to[tile] == 0 && row < g.n_q) {
+    if (my_to == 0 && row < g.n_q) {  // every row of the tile sees nothing
         uint16_t* orow = g.out + row * uint64_t(g.ldo) + uint64_t(head) * g.dim;
         for (int c = 0; c < g.dim; c += 8) *reinterpret_cast<uint4*>(orow + c) = make_uint4(0, 0, 0, 0);
         if (g.lse) g.lse[row * g.heads + head] = -INFINITY;
+    }
     }
     fence_before();
     __syncthreads();
@@ -506,8 +515,9 @@ int launch(const AttnArgs& g, const CUtensorMap& q, const CUtensorMap& k, const 
     constexpr int smem = (2 + 2 * kSt) * kRows * DP * 2 + 1024 + 512;
     auto kern = attention_kernel<DP, CAP, BIAS>;
     GATB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    const dim3 grid(unsigned((g.n_q + 2 * kRows - 1) / (2 * kRows)), unsigned(g.heads));
-    kern<<<grid, kThreads, smem, st>>>(q, k, v, g);
+    const uint64_t grid = (g.n_q + 2 * kRows - 1) / (2 * kRows) * uint64_t(g.heads);
+    if (grid > uint64_t(INT32_MAX)) return fail("masked_attention: too many rows times heads");
+    kern<<<unsigned(grid), kThreads, smem, st>>>(q, k, v, g);
     GATB_LAUNCH("masked_attention kernel");
     return 0;
 }
