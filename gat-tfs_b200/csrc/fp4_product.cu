@@ -4,11 +4,11 @@
 // tensor core, out of tensor memory, where tcgen05.cp brings them from shared
 // memory in the tables' own tile order (fp4.cuh).
 //
-// Persistent kernel, one CTA per SM, 6 warps:
-//   warp 0  TMA producer: stages of 256 columns (128 bytes a row, 128-byte
-//           swizzle) of 128 rows of a and of b with their scale tiles.
-//   warp 1  scale copies and MMAs into one of two TMEM accumulators.
-//   warps 2-5 epilogue: TMEM -> row scales -> rounding -> global.
+// Two kernels; fp4_product_launch chooses by the number of output tiles.
+//  pair_kernel  256 x 256 tiles of a CTA pair (cta_group::2), persistent, for
+//               outputs of at least a wave of such tiles.
+//  rows_kernel  128 rows of b x BN rows of a, the reduction split over a cluster
+//               and joined through distributed shared memory: few rows, small outputs.
 // Every wait is bounded (GAT_B200_ETIMEOUT through gat_b200_check_device).
 #include <cuda.h>
 
@@ -27,10 +27,6 @@ namespace {
 
 using namespace tc;
 
-constexpr int kBM = 128, kBN = 128;
-constexpr int kStages = 5;
-constexpr int kThreads = 192;
-
 struct ProductArgs {
     uint64_t m;
     int n;
@@ -44,48 +40,347 @@ struct ProductArgs {
     void* out;
     int ldo;
     int out_bf16;
+    int tma_out;  // output rows are 16-byte aligned: tiles leave through TMA stores
+    int n_whole;  // n columns are whole 16-byte pieces
     uint32_t grid_m, grid_n;
 };
 
+// MMAs served by one 4-block scale tile, scale tiles of a 256-column stage.
 template <int FORMAT>
-__global__ void __launch_bounds__(kThreads, 1)
-    fp4_product_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                       const __grid_constant__ ProductArgs g) {
-    constexpr bool kMx = FORMAT == GAT_B200_MXFP4;
-    constexpr int kTileMmas = kMx ? 2 : 1;           // MMAs served by one scale tile
-    constexpr int kSfTiles = 4 / kTileMmas;          // scale tiles of a stage
-    constexpr int kABytes = kBM * 128, kBBytes = kBN * 128, kSfBytes = kSfTiles * 512;
-    constexpr int kStageBytes = kABytes + kBBytes + 2 * kSfBytes;
+struct Scales {
+    static constexpr bool kMx = FORMAT == GAT_B200_MXFP4;
+    static constexpr int kTileMmas = kMx ? 2 : 1;
+    static constexpr int kTiles = 4 / kTileMmas;
+    static constexpr int kBytes = kTiles * 512;  // of 128 rows in a stage
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t saddr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void mbar_arrive_rank(uint64_t* bar, uint32_t rank) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_to_rank(smem_u32(bar), rank))
+                 : "memory");
+}
+// Loads of a CTA pair count on the first CTA's barrier (bit 24 of a shared
+// address holds the CTA's parity in the pair).
+__device__ __forceinline__ void pair_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+        "[%2];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(smem_u32(bar) & 0xfeffffffu), "r"(x), "r"(y)
+        : "memory");
+}
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(uint16_t(3))
+        : "memory");
+}
+
+// ------------------------------------------------------------ CTA pairs
+// Roles of the 10 warps of each CTA of a pair:
+//   warp 0    TMA producer: this CTA's 128 rows of a, 128 of the tile's 256 rows
+//             of b (the pair's MMA reads both halves) and their scales; the
+//             scales of b's whole tile, which each CTA's tensor memory holds.
+//   warp 1    first CTA only: scale copies and MMAs of the pair.
+//   warps 2-9 epilogue of this CTA's 128 x 256 accumulators.
+// Tensor memory: accumulators of even tiles in columns 0-255, of odd tiles in
+// 192-447, scales in 448-511. Two whole accumulators and the scales do not fit,
+// so they share 64 columns, which the epilogue drains first: the next tile's
+// MMAs start while three quarters of this one still leave.
+constexpr int kPairThreads = 320;
+constexpr int kPairStages = 4;
+constexpr int kOdd = 192, kScaleCols = 448;
+
+template <int FORMAT>
+__global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                const __grid_constant__ CUtensorMap tm_sa, const __grid_constant__ CUtensorMap tm_sb,
+                const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ ProductArgs g) {
+    using S = Scales<FORMAT>;
+    constexpr int kHalf = 128 * 128;  // codes of 128 rows in a stage
+    constexpr int kStage = 2 * kHalf + 3 * S::kBytes;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* sf_s = smem + size_t(kStages) * (kABytes + kBBytes);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + size_t(kStages) * kStageBytes);
+    uint8_t* st_s = smem + kPairStages * 2 * kHalf;               // 8 warps x 2 x 4 KB
+    uint8_t* sf_s = st_s + 8 * 2 * 4096;                           // stages x 3 scale pieces
+    float* rb_s = reinterpret_cast<float*>(sf_s + kPairStages * 3 * S::kBytes);  // 8 warps x 64
+    uint64_t* bars = reinterpret_cast<uint64_t*>(rb_s + 8 * 64);
     uint64_t* full = bars;
-    uint64_t* empty = bars + kStages;
-    uint64_t* acc_full = bars + 2 * kStages;  // [2]
-    uint64_t* acc_empty = acc_full + 2;       // [2]
-    uint64_t* mma_done = acc_empty + 2;
+    uint64_t* empty = full + kPairStages;
+    uint64_t* acc_full = empty + kPairStages;  // [2]
+    uint64_t* drained = acc_full + 2;
+    uint64_t* mma_done = drained + 1;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(mma_done + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
     const uint32_t ntiles = g.grid_m * g.grid_n;
+    const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    // 8 row tiles by all column tiles at a time, so that the tiles in flight share rows and columns in L2
+    auto tile_at = [&](uint32_t t, uint32_t& tm, uint32_t& tn) {
+        const uint32_t per = 8 * g.grid_n, grp = t / per, in = t % per;
+        const uint32_t rows = min(8u, g.grid_m - grp * 8);
+        tm = grp * 8 + in % rows;
+        tn = in / rows;
+    };
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
+        for (int s = 0; s < kPairStages; ++s) {
             mbar_init(full + s, 1);
             mbar_init(empty + s, 1);
         }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(acc_full + b, 1);
-            mbar_init(acc_empty + b, 4);
-        }
+        mbar_init(acc_full + 0, 1);
+        mbar_init(acc_full + 1, 1);
+        mbar_init(drained, 16);
         mbar_init(mma_done, 1);
         *abort_flag = 0;
         fence_mbarrier_init();
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
                      "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    cluster_sync();
+    fence_after();
+    const uint32_t tmem = *tmem_holder;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t kc = 0;
+            bool ok = true;
+            for (uint32_t t = pair; t < ntiles && ok; t += pairs) {
+                uint32_t tm, tn;
+                tile_at(t, tm, tn);
+                const int arow = int(tm * 256 + rank * 128), brow = int(tn * 256 + rank * 128);
+                for (int k = 0; k < g.stages_k; ++k, ++kc) {
+                    const int s = int(kc % kPairStages);
+                    if (!mbar_wait(empty + s, ((kc / kPairStages) & 1u) ^ 1u, abort_flag, &g_fp4_error)) { ok = false; break; }
+                    if (rank == 0) mbar_expect_tx(full + s, 2 * kStage);
+                    uint8_t* c = smem + s * 2 * kHalf;
+                    uint8_t* f = sf_s + s * 3 * S::kBytes;
+                    pair_load_2d(c, &tm_a, full + s, k * 128, arow);
+                    pair_load_2d(c + kHalf, &tm_b, full + s, k * 128, brow);
+                    // boxes of a stage's scale tiles; past a row's last tile they hold what no MMA uses
+                    pair_load_2d(f, &tm_sa, full + s, 0, int((tm * 2 + rank) * g.tiles) + k * S::kTiles);
+                    pair_load_2d(f + S::kBytes, &tm_sb, full + s, 0, int(tn * 2 * g.tiles) + k * S::kTiles);
+                    pair_load_2d(f + 2 * S::kBytes, &tm_sb, full + s, 0, int((tn * 2 + 1) * g.tiles) + k * S::kTiles);
+                }
+            }
+            // every load has landed once its stage came back (or, at the first CTA, filled)
+            for (uint32_t i = kc > kPairStages ? kc - kPairStages : 0; i < kc; ++i)
+                mbar_wait(empty + i % kPairStages, (i / kPairStages) & 1u, abort_flag, &g_fp4_error);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            uint32_t kc = 0, tl = 0;
+            bool ok = true;
+            const uint32_t sfa0 = tmem + kScaleCols, sfb0 = sfa0 + 4 * S::kTiles;
+            for (uint32_t t = pair; t < ntiles && ok; t += pairs, ++tl) {
+                if (tl && !mbar_wait(drained, (tl - 1) & 1u, abort_flag, &g_fp4_error)) { ok = false; break; }
+                fence_after();
+                const uint32_t d = tmem + ((tl & 1u) ? kOdd : 0);
+                for (int k = 0; k < g.stages_k; ++k, ++kc) {
+                    const int s = int(kc % kPairStages);
+                    if (!mbar_wait(full + s, (kc / kPairStages) & 1u, abort_flag, &g_fp4_error)) { ok = false; break; }
+                    fence_after();
+                    const uint32_t a_addr = smem_u32(smem + s * 2 * kHalf), b_addr = a_addr + kHalf;
+                    const uint32_t f = smem_u32(sf_s + s * 3 * S::kBytes);
+                    const int mmas = k + 1 == g.stages_k ? g.last_mmas : 4;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (j >= mmas) break;
+                        const int st = j / S::kTileMmas;
+                        const uint32_t sfa = sfa0 + st * 4, sfb = sfb0 + st * 8;
+                        if (j % S::kTileMmas == 0) {
+                            tmem_cp_scales<2>(sfa, desc_scales(f + st * 512));
+                            tmem_cp_scales<2>(sfb, desc_scales(f + S::kBytes + st * 512));
+                            tmem_cp_scales<2>(sfb + 4, desc_scales(f + 2 * S::kBytes + st * 512));
+                        }
+                        mma_fp4<S::kMx, 2>(d, desc_sw128(a_addr + j * 32, 16, 1024), desc_sw128(b_addr + j * 32, 16, 1024),
+                                           idesc_fp4(256, 256, S::kMx, S::kMx ? 2 * (j & 1) : 0), sfa, sfb,
+                                           (k | j) ? 1u : 0u);
+                    }
+                    pair_commit(empty + s);
+                }
+                if (!ok) break;
+                pair_commit(acc_full + (tl & 1u));
+            }
+            pair_commit(mma_done);
+            mbar_wait(mma_done, 0, abort_flag, &g_fp4_error);
+        }
+    } else {
+        const int q = warp & 3, ew = warp - 2, set = ew >> 2;
+        uint8_t* stage = st_s + ew * 2 * 4096;
+        float* rb = rb_s + ew * 64;
+        uint32_t tl = 0, toggle = 0;
+        for (uint32_t t = pair; t < ntiles; t += pairs, ++tl) {
+            uint32_t tm, tn;
+            tile_at(t, tm, tn);
+            const uint32_t odd = tl & 1u;
+            if (!mbar_wait(acc_full + odd, (tl >> 1) & 1u, abort_flag, &g_fp4_error)) break;
+            fence_after();
+            const uint32_t acc = tmem + (odd ? kOdd : 0) + (uint32_t(q * 32) << 16);
+            const uint64_t row0 = uint64_t(tm) * 256 + rank * 128 + q * 32;
+            const float ra = g.a_row && row0 + lane < g.m ? g.a_row[row0 + lane] : 1.f;
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i) {
+                // 64-column groups in the order 3 2 | 1 0 (even tiles) and 0 1 | 2 3 (odd tiles) of the two sets
+                const int grp = odd ? 2 * set + i : 3 - 2 * set - i;
+                const int col = int(tn) * 256 + grp * 64;
+                if (g.b_row) {
+                    __syncwarp();
+                    rb[lane] = col + lane < g.n ? g.b_row[col + lane] : 0.f;
+                    rb[lane + 32] = col + lane + 32 < g.n ? g.b_row[col + lane + 32] : 0.f;
+                    __syncwarp();
+                }
+                float v[64];
+                tmem_ld64(acc + grp * 64, v);
+                // the shared columns are in registers (set 0), everything is (set 1)
+                if (i == set) {
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_rank(drained, 0);
+                }
+                if (col >= g.n || row0 >= g.m) continue;
+                if (g.b_row) {
+#pragma unroll
+                    for (int c = 0; c < 64; c += 4) {
+                        const float4 b4 = *reinterpret_cast<const float4*>(rb + c);
+                        v[c] *= ra * b4.x;
+                        v[c + 1] *= ra * b4.y;
+                        v[c + 2] *= ra * b4.z;
+                        v[c + 3] *= ra * b4.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 64; ++c) v[c] *= ra;
+                }
+                // 32 rows x 128 bytes at a time, 16-byte pieces swizzled as the TMA store expects
+                const int halves = g.out_bf16 ? 1 : 2;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (h >= halves || col + 32 * h >= g.n) break;
+                    uint8_t* sb = stage + toggle * 4096;
+                    toggle ^= 1u;
+                    if (lane == 0 && g.tma_out) bulk_wait_read<1>();
+                    __syncwarp();
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        uint4 w;
+                        if (g.out_bf16) {
+                            w = make_uint4(pack_bf16x2(v[8 * c], v[8 * c + 1]), pack_bf16x2(v[8 * c + 2], v[8 * c + 3]),
+                                           pack_bf16x2(v[8 * c + 4], v[8 * c + 5]), pack_bf16x2(v[8 * c + 6], v[8 * c + 7]));
+                        } else {
+                            w = make_uint4(__float_as_uint(v[32 * h + 4 * c]), __float_as_uint(v[32 * h + 4 * c + 1]),
+                                           __float_as_uint(v[32 * h + 4 * c + 2]), __float_as_uint(v[32 * h + 4 * c + 3]));
+                        }
+                        *reinterpret_cast<uint4*>(sb + lane * 128 + ((c ^ (lane & 7)) * 16)) = w;
+                    }
+                    // a TMA store writes whole 16-byte pieces: the last columns go out one by one unless n ends a piece
+                    if (g.tma_out && (g.n_whole || col + 32 * h + (g.out_bf16 ? 64 : 32) <= g.n)) {
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_2d(&tm_out, sb, col + 32 * h, int(row0));
+                            bulk_commit();
+                        }
+                    } else {
+                        if (lane == 0) bulk_commit();  // an empty group: the two buffers keep their turns
+                        __syncwarp();
+                        const int width = g.out_bf16 ? 64 : 32;
+                        for (int r = 0; r < 32 && row0 + r < g.m; ++r)
+                            for (int c = lane; c < width && col + 32 * h + c < g.n; c += 32) {
+                                const int byte = c * (g.out_bf16 ? 2 : 4);
+                                const uint8_t* src = sb + r * 128 + (((byte >> 4) ^ (r & 7)) * 16) + (byte & 15);
+                                const uint64_t off = (row0 + r) * uint64_t(g.ldo) + col + 32 * h + c;
+                                if (g.out_bf16)
+                                    static_cast<uint16_t*>(g.out)[off] = *reinterpret_cast<const uint16_t*>(src);
+                                else
+                                    static_cast<float*>(g.out)[off] = *reinterpret_cast<const float*>(src);
+                            }
+                    }
+                }
+            }
+        }
+        if (lane == 0) bulk_wait_all();
+        __syncwarp();
+    }
+    fence_before();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+// ------------------------------------------------------------- few rows
+// out^T: 128 rows of b (an MMA's M) x BN rows of a (its N). The SPLIT CTAs of a
+// cluster take a part of the reduction each, leave their FP32 tile in shared
+// memory, and each sums a share of the tile's columns over the cluster in rank
+// order, so results do not depend on timing. 6 warps: producer, MMA, 4 epilogue.
+constexpr int kRowsThreads = 192;
+
+template <int BN>
+struct RowsTile {
+    static constexpr int kStages = 4;
+    static constexpr int kCols = BN <= 16 ? 32 : BN;  // accumulator columns, up to 32 of scales behind them
+    static constexpr int kTmem = BN <= 32 ? 64 : (BN <= 64 ? 128 : 256);
+};
+
+template <int FORMAT, int BN>
+__global__ void __launch_bounds__(kRowsThreads)
+    rows_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                const __grid_constant__ ProductArgs g, const int split) {
+    using S = Scales<FORMAT>;
+    constexpr int kSt = RowsTile<BN>::kStages, kTmem = RowsTile<BN>::kTmem;
+    constexpr int kB = 128 * 128, kA = BN * 128;  // codes of a stage: b's rows, a's rows
+    constexpr int kStage = kB + kA + 2 * S::kBytes;
+    constexpr int kPitch = 128 + 4;               // floats of a column of out^T in the exchange buffer
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* a_s = smem + kSt * kB;
+    uint8_t* sf_s = a_s + kSt * kA;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSt * kStage);
+    uint64_t* full = bars;
+    uint64_t* empty = full + kSt;
+    uint64_t* acc_full = empty + kSt;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_full + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+    float* part = reinterpret_cast<float*>(smem);  // [BN][kPitch], over the stages once they are used up
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = split > 1 ? cluster_rank() : 0;
+    const uint32_t tile = blockIdx.x / split;
+    const uint32_t tn = tile % g.grid_n, tm = tile / g.grid_n;  // 128 rows of b, BN rows of a
+    const int k0 = int(uint64_t(g.stages_k) * rank / split), k1 = int(uint64_t(g.stages_k) * (rank + 1) / split);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kSt; ++s) {
+            mbar_init(full + s, 1);
+            mbar_init(empty + s, 1);
+        }
+        mbar_init(acc_full, 1);
+        *abort_flag = 0;
+        fence_mbarrier_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                     "r"(kTmem));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     fence_before();
@@ -95,110 +390,111 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 0) {
         if (lane == 0) {
-            uint32_t kc = 0;
-            bool ok = true;
-            for (uint32_t t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
-                const uint32_t tm = t % g.grid_m, tn = t / g.grid_m;
-                for (int k = 0; k < g.stages_k; ++k, ++kc) {
-                    const int s = int(kc % kStages);
-                    if (!mbar_wait(empty + s, ((kc / kStages) & 1u) ^ 1u, abort_flag, &g_fp4_error)) { ok = false; break; }
-                    const int sft = min(kSfTiles, g.tiles - k * kSfTiles);
-                    mbar_expect_tx(full + s, kABytes + kBBytes + 2 * 512 * sft);
-                    uint8_t* a_s = smem + size_t(s) * (kABytes + kBBytes);
-                    tma_load_2d(a_s, &tm_a, full + s, k * 128, int(tm * kBM));
-                    tma_load_2d(a_s + kABytes, &tm_b, full + s, k * 128, int(tn * kBN));
-                    uint8_t* sf = sf_s + size_t(s) * 2 * kSfBytes;
-                    bulk_load(sf, g.a_scales + (uint64_t(tm) * g.tiles + k * kSfTiles) * 512, 512 * sft, full + s);
-                    bulk_load(sf + kSfBytes, g.b_scales + (uint64_t(tn) * g.tiles + k * kSfTiles) * 512, 512 * sft, full + s);
-                }
+            const uint64_t arow = uint64_t(tm) * BN;
+            int k = k0;
+            for (; k < k1; ++k) {
+                const int i = k - k0, s = i % kSt;
+                if (!mbar_wait(empty + s, ((uint32_t(i) / kSt) & 1u) ^ 1u, abort_flag, &g_fp4_error)) break;
+                const int sft = min(S::kTiles, g.tiles - k * S::kTiles);
+                mbar_expect_tx(full + s, kB + kA + 2 * 512 * sft);
+                tma_load_2d(smem + s * kB, &tm_b, full + s, k * 128, int(tn * 128));
+                tma_load_2d(a_s + s * kA, &tm_a, full + s, k * 128, int(arow));
+                uint8_t* f = sf_s + s * 2 * S::kBytes;
+                bulk_load(f, g.b_scales + (uint64_t(tn) * g.tiles + k * S::kTiles) * 512, 512 * sft, full + s);
+                bulk_load(f + S::kBytes, g.a_scales + ((arow >> 7) * uint64_t(g.tiles) + k * S::kTiles) * 512, 512 * sft, full + s);
             }
-            for (int s = 0; s < kStages; ++s)
-                if (kc > uint32_t(s)) {
-                    const uint32_t last = kc - 1 - ((kc - 1 - s) % kStages);
-                    mbar_wait(full + s, (last / kStages) & 1u, abort_flag, &g_fp4_error);
-                }
+            for (int i = max(0, k - k0 - kSt); i < k - k0; ++i)
+                mbar_wait(full + i % kSt, (uint32_t(i) / kSt) & 1u, abort_flag, &g_fp4_error);
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            uint32_t kc = 0, tl = 0;
-            bool ok = true;
-            const uint32_t sf_t = tmem + 256;
-            for (uint32_t t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++tl) {
-                const uint32_t buf = tl & 1u;
-                if (!mbar_wait(acc_empty + buf, ((tl >> 1) & 1u) ^ 1u, abort_flag, &g_fp4_error)) { ok = false; break; }
+            // scales behind the accumulator; a's rows start a scale tile (below 128 rows there is one tile of them)
+            const uint32_t sfb0 = tmem + RowsTile<BN>::kCols, sfa0 = sfb0 + 4 * S::kTiles;
+            for (int k = k0; k < k1; ++k) {
+                const int i = k - k0, s = i % kSt;
+                if (!mbar_wait(full + s, (uint32_t(i) / kSt) & 1u, abort_flag, &g_fp4_error)) break;
                 fence_after();
-                const uint32_t d = tmem + buf * 128;
-                for (int k = 0; k < g.stages_k; ++k, ++kc) {
-                    const int s = int(kc % kStages);
-                    if (!mbar_wait(full + s, (kc / kStages) & 1u, abort_flag, &g_fp4_error)) { ok = false; break; }
-                    fence_after();
-                    const uint32_t a_addr = smem_u32(smem + size_t(s) * (kABytes + kBBytes));
-                    const uint32_t b_addr = a_addr + kABytes;
-                    const uint32_t sfa_s = smem_u32(sf_s + size_t(s) * 2 * kSfBytes), sfb_s = sfa_s + kSfBytes;
-                    const int mmas = k + 1 == g.stages_k ? g.last_mmas : 4;
-                    const uint32_t sfa = sf_t + (kc & 1u) * (8 * kSfTiles), sfb = sfa + 4 * kSfTiles;
+                const uint32_t b_addr = smem_u32(smem + s * kB), a_addr = smem_u32(a_s + s * kA);
+                const uint32_t f = smem_u32(sf_s + s * 2 * S::kBytes);
+                const int mmas = k + 1 == g.stages_k ? g.last_mmas : 4;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (j >= mmas) break;
-                        const int st = j / kTileMmas;
-                        if (j % kTileMmas == 0) {
-                            tmem_cp_scales<1>(sfa + st * 4, desc_scales(sfa_s + st * 512));
-                            tmem_cp_scales<1>(sfb + st * 4, desc_scales(sfb_s + st * 512));
-                        }
-                        mma_fp4<kMx, 1>(d, desc_sw128(a_addr + j * 32, 16, 1024), desc_sw128(b_addr + j * 32, 16, 1024),
-                                        idesc_fp4(kBM, kBN, kMx, kMx ? 2 * (j & 1) : 0), sfa + st * 4, sfb + st * 4,
-                                        (k | j) ? 1u : 0u);
+                for (int j = 0; j < 4; ++j) {
+                    if (j >= mmas) break;
+                    const int st = j / S::kTileMmas;
+                    if (j % S::kTileMmas == 0) {
+                        tmem_cp_scales<1>(sfb0 + st * 4, desc_scales(f + st * 512));
+                        tmem_cp_scales<1>(sfa0 + st * 4, desc_scales(f + S::kBytes + st * 512));
                     }
-                    mma_commit(empty + s);
+                    mma_fp4<S::kMx, 1>(tmem, desc_sw128(b_addr + j * 32, 16, 1024), desc_sw128(a_addr + j * 32, 16, 1024),
+                                       idesc_fp4(128, BN, S::kMx, S::kMx ? 2 * (j & 1) : 0), sfb0 + st * 4,
+                                       sfa0 + st * 4, (i | j) ? 1u : 0u);
                 }
-                if (!ok) break;
-                mma_commit(acc_full + buf);
+                mma_commit(empty + s);
             }
-            mma_commit(mma_done);
-            mbar_wait(mma_done, 0, abort_flag, &g_fp4_error);
-        }
-    } else {
-        const int q = warp & 3;
-        uint32_t tl = 0;
-        for (uint32_t t = blockIdx.x; t < ntiles; t += gridDim.x, ++tl) {
-            const uint32_t tm = t % g.grid_m, tn = t / g.grid_m;
-            const uint32_t buf = tl & 1u;
-            if (!mbar_wait(acc_full + buf, (tl >> 1) & 1u, abort_flag, &g_fp4_error)) break;
-            fence_after();
-            const uint64_t row = uint64_t(tm) * kBM + q * 32 + lane;
-            const float ra = g.a_row && row < g.m ? g.a_row[row] : 1.f;
-#pragma unroll
-            for (int c = 0; c < kBN; c += 32) {
-                float v[32];
-                tmem_ld32(tmem + buf * 128 + (uint32_t(q * 32) << 16) + c, v);
-                const int col = int(tn) * kBN + c;
-                if (row < g.m) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (col + j < g.n) {
-                            const float y = g.b_row ? v[j] * ra * __ldg(g.b_row + col + j) : v[j] * ra;
-                            const uint64_t off = row * uint64_t(g.ldo) + col + j;
-                            if (g.out_bf16)
-                                static_cast<uint16_t*>(g.out)[off] = uint16_t(pack_bf16x2(y, 0.f));
-                            else
-                                static_cast<float*>(g.out)[off] = y;
-                        }
-                }
-                __syncwarp();
-            }
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty + buf);
+            mma_commit(acc_full);
+            mbar_wait(acc_full, 0, abort_flag, &g_fp4_error);
         }
     }
-    fence_before();
+    // the accumulator is complete; nobody reads the stages any more
+    bool ok = k1 > k0;
+    if (warp >= 2 && ok) ok = mbar_wait(acc_full, 0, abort_flag, &g_fp4_error);
     __syncthreads();
+    const int q = warp & 3;
+    const int col = int(tn) * 128 + q * 32 + lane;  // output column: a row of b
+    const uint64_t arow = uint64_t(tm) * BN;
+    const int rows = int(min(uint64_t(BN), g.m - arow));
+    auto store = [&](int r, float y) {
+        const uint64_t off = (arow + r) * uint64_t(g.ldo) + col;
+        if (g.out_bf16)
+            static_cast<uint16_t*>(g.out)[off] = uint16_t(pack_bf16x2(y, 0.f));
+        else
+            static_cast<float*>(g.out)[off] = y;
+    };
+    if (warp >= 2) {
+        fence_after();
+        const float rb = g.b_row && col < g.n ? g.b_row[col] : 1.f;
+#pragma unroll 1
+        for (int c = 0; c < BN; c += 16) {
+            if (c >= rows) break;
+            float v[16];
+            tmem_ld16(tmem + (uint32_t(q * 32) << 16) + c, v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float y = ok ? v[i] : 0.f;  // a CTA without columns of the reduction adds nothing
+                if (split > 1)
+                    part[(c + i) * kPitch + q * 32 + lane] = y;
+                else if (c + i < rows && col < g.n)
+                    store(c + i, g.a_row ? y * (rb * g.a_row[arow + c + i]) : y * rb);
+            }
+        }
+        fence_before();
+    }
+    if (split > 1) {
+        cluster_sync();
+        if (warp >= 2) {
+            const float rb = g.b_row && col < g.n ? g.b_row[col] : 1.f;
+            for (int r = int(rank); r < rows; r += split) {
+                const uint32_t at = smem_u32(part + r * kPitch + q * 32 + lane);
+                float y = 0.f;
+                for (int c = 0; c < split; ++c) {
+                    float x;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(map_to_rank(at, uint32_t(c))));
+                    y += x;
+                }
+                if (col < g.n) store(r, g.a_row ? y * (rb * g.a_row[arow + r]) : y * rb);
+            }
+        }
+        cluster_sync();  // the others have read this CTA's part
+    } else {
+        __syncthreads();
+    }
     if (warp == 1) {
         fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmem));
     }
 }
 
+// ---- host side -------------------------------------------------------------
 // Codes as bytes: rows of `row_bytes`, boxes of 128 bytes x `box_rows` rows.
 int codes_map(CUtensorMap* m, const void* base, uint64_t rows, int row_bytes, int ld, uint32_t box_rows) {
     const uint64_t dims[2] = {uint64_t(row_bytes), rows};
@@ -206,17 +502,89 @@ int codes_map(CUtensorMap* m, const void* base, uint64_t rows, int row_bytes, in
     const uint32_t box[2] = {128, box_rows};
     return make_tiled_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, true);
 }
+// Scale tiles as rows of 512 bytes, boxes of a stage's tiles.
+int scales_map(CUtensorMap* m, const void* base, uint64_t rows, int tiles, uint32_t box_tiles) {
+    const uint64_t dims[2] = {128, (rows + 127) / 128 * uint64_t(tiles)};
+    const uint64_t strides[1] = {512};
+    const uint32_t box[2] = {128, box_tiles};
+    return make_tiled_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, base, dims, strides, box, false);
+}
 
 template <int FORMAT>
-int launch_product(const ProductArgs& g, const CUtensorMap& tm_a, const CUtensorMap& tm_b, int sms, cudaStream_t st) {
-    constexpr int sf = FORMAT == GAT_B200_MXFP4 ? 1024 : 2048;
-    const size_t smem = size_t(kStages) * (kBM * 128 + kBN * 128 + 2 * sf) + 256 + 1024;
-    auto kern = fp4_product_kernel<FORMAT>;
-    GATB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-    const uint32_t ntiles = g.grid_m * g.grid_n;
-    kern<<<ntiles < uint32_t(sms) ? ntiles : sms, kThreads, smem, st>>>(tm_a, tm_b, g);
-    GATB_LAUNCH("fp4_product kernel");
+int launch_pair(ProductArgs g, const void* a, int lda, const void* b, int ldb, int kb, int sms, cudaStream_t st) {
+    using S = Scales<FORMAT>;
+    g.grid_m = uint32_t((g.m + 255) / 256);
+    g.grid_n = uint32_t((g.n + 255) / 256);
+    CUtensorMap tm_a, tm_b, tm_sa, tm_sb, tm_out;
+    if (int rc = codes_map(&tm_a, a, g.m, kb, lda, 128)) return rc;
+    if (int rc = codes_map(&tm_b, b, uint64_t(g.n), kb, ldb, 128)) return rc;
+    if (int rc = scales_map(&tm_sa, g.a_scales, g.m, g.tiles, S::kTiles)) return rc;
+    if (int rc = scales_map(&tm_sb, g.b_scales, uint64_t(g.n), g.tiles, S::kTiles)) return rc;
+    const int es = g.out_bf16 ? 2 : 4;
+    g.tma_out = (reinterpret_cast<uintptr_t>(g.out) | (uint64_t(g.ldo) * es)) % 16 == 0;
+    g.n_whole = uint64_t(g.n) * es % 16 == 0;
+    if (g.tma_out) {
+        const uint64_t dims[2] = {uint64_t(g.n), g.m};
+        const uint64_t strides[1] = {uint64_t(g.ldo) * es};
+        const uint32_t box[2] = {uint32_t(128 / es), 32};
+        if (int rc = make_tiled_map(&tm_out, g.out_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                                    2, g.out, dims, strides, box, true))
+            return rc;
+    } else {
+        tm_out = tm_a;  // not used
+    }
+    constexpr int smem = kPairStages * (2 * 16384 + 3 * S::kBytes) + 8 * 2 * 4096 + 8 * 64 * 4 + 256 + 1024;
+    auto kern = pair_kernel<FORMAT>;
+    GATB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    const uint64_t ntiles = uint64_t(g.grid_m) * g.grid_n;
+    const unsigned pairs = unsigned(ntiles < uint64_t(sms / 2) ? ntiles : uint64_t(sms / 2));
+    kern<<<2 * pairs, kPairThreads, smem, st>>>(tm_a, tm_b, tm_sa, tm_sb, tm_out, g);
+    GATB_LAUNCH("fp4_product (pair) kernel");
     return 0;
+}
+
+template <int FORMAT, int BN>
+int launch_rows(ProductArgs g, const void* a, int lda, const void* b, int ldb, int kb, int sms, cudaStream_t st) {
+    using S = Scales<FORMAT>;
+    g.grid_m = uint32_t((g.m + BN - 1) / BN);
+    g.grid_n = uint32_t((g.n + 127) / 128);
+    const uint64_t tiles = uint64_t(g.grid_m) * g.grid_n;
+    // split the reduction while that leaves CTAs for idle SMs and each part two stages
+    int split = 1;
+    while (split < 8 && tiles * split < uint64_t(sms) && g.stages_k >= 4 * split) split *= 2;
+    CUtensorMap tm_a, tm_b;
+    if (int rc = codes_map(&tm_a, a, g.m, kb, lda, BN)) return rc;
+    if (int rc = codes_map(&tm_b, b, uint64_t(g.n), kb, ldb, 128)) return rc;
+    constexpr int stages = RowsTile<BN>::kStages * (128 * 128 + BN * 128 + 2 * S::kBytes);
+    constexpr int part = BN * 132 * 4;
+    static_assert(part <= stages, "the exchange buffer lies over the stages");
+    constexpr int smem = stages + 256 + 1024;
+    auto kern = rows_kernel<FORMAT, BN>;
+    GATB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(tiles * split));
+    cfg.blockDim = dim3(kRowsThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = unsigned(split);
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    GATB_CUDA(cudaLaunchKernelEx(&cfg, kern, tm_a, tm_b, g, split));
+    return 0;
+}
+
+template <int FORMAT>
+int launch_product(const ProductArgs& g, const void* a, int lda, const void* b, int ldb, int kb, int sms,
+                   cudaStream_t st) {
+    const uint64_t pair_tiles = (g.m + 255) / 256 * ((uint64_t(g.n) + 255) / 256);
+    if (pair_tiles >= uint64_t(sms / 2)) return launch_pair<FORMAT>(g, a, lda, b, ldb, kb, sms, st);
+    if (g.m <= 16) return launch_rows<FORMAT, 16>(g, a, lda, b, ldb, kb, sms, st);
+    if (g.m <= 32) return launch_rows<FORMAT, 32>(g, a, lda, b, ldb, kb, sms, st);
+    if (g.m <= 64) return launch_rows<FORMAT, 64>(g, a, lda, b, ldb, kb, sms, st);
+    return launch_rows<FORMAT, 128>(g, a, lda, b, ldb, kb, sms, st);
 }
 
 }  // namespace
@@ -227,7 +595,7 @@ int fp4_product_launch(int format, uint64_t m, int n, int k, const void* a, int 
     if (int rc = fp4_check_format("fp4_product", format)) return rc;
     if (out_dtype != GAT_B200_F32 && out_dtype != GAT_B200_BF16) return fail("fp4_product: bad output dtype");
     if (n < 0 || k <= 0 || k > (1 << 24)) return fail("fp4_product: bad shape");
-    if (m > uint64_t(INT32_MAX - 256) || n > INT32_MAX - 256) return fail("fp4_product: too many rows");
+    if (m > uint64_t(INT32_MAX - 512) || n > INT32_MAX - 512) return fail("fp4_product: too many rows");
     const int kb = fp4_row_bytes(k);
     if (lda < kb || lda % 16 || ldb < kb || ldb % 16)
         return fail("fp4_product: code rows must be 16-byte aligned and hold the width");
@@ -240,13 +608,17 @@ int fp4_product_launch(int format, uint64_t m, int n, int k, const void* a, int 
     if (reinterpret_cast<uintptr_t>(out) % (out_dtype == GAT_B200_BF16 ? 2 : 4) ||
         (reinterpret_cast<uintptr_t>(a_row) | reinterpret_cast<uintptr_t>(b_row)) % 4)
         return fail("fp4_product: misaligned pointer");
-    if (int rc = check_device_pointers("fp4_product", {a, a_scales, a_row, b, b_scales, b_row, out})) return rc;
     ProductArgs g{};
     g.m = m;
     g.n = n;
     g.stages_k = (kb + 127) / 128;
     g.last_mmas = (k - (g.stages_k - 1) * 256 + 63) / 64;
     g.tiles = fp4_tiles(format, k);
+    // scale tiles are counted in 32 bits (TMA rows), output tiles as a grid
+    if (((m > uint64_t(n) ? m : uint64_t(n)) + 511) / 128 * uint64_t(g.tiles) > uint64_t(INT32_MAX) ||
+        (m + 15) / 16 * ((uint64_t(n) + 127) / 128) * 8 > uint64_t(INT32_MAX))
+        return fail("fp4_product: tables too large");
+    if (int rc = check_device_pointers("fp4_product", {a, a_scales, a_row, b, b_scales, b_row, out})) return rc;
     g.a_scales = static_cast<const uint8_t*>(a_scales);
     g.b_scales = static_cast<const uint8_t*>(b_scales);
     g.a_row = a_row;
@@ -254,17 +626,11 @@ int fp4_product_launch(int format, uint64_t m, int n, int k, const void* a, int 
     g.out = out;
     g.ldo = ldo;
     g.out_bf16 = out_dtype == GAT_B200_BF16;
-    g.grid_m = uint32_t((m + kBM - 1) / kBM);
-    g.grid_n = uint32_t((n + kBN - 1) / kBN);
-    if (uint64_t(g.grid_m) * g.grid_n > uint64_t(INT32_MAX)) return fail("fp4_product: output too large");
     int dev = 0, sms = 0;
     GATB_CUDA(cudaGetDevice(&dev));
     GATB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    CUtensorMap tm_a, tm_b;
-    if (int rc = codes_map(&tm_a, a, m, kb, lda, kBM)) return rc;
-    if (int rc = codes_map(&tm_b, b, uint64_t(n), kb, ldb, kBN)) return rc;
-    return format == GAT_B200_MXFP4 ? launch_product<GAT_B200_MXFP4>(g, tm_a, tm_b, sms, st)
-                                    : launch_product<GAT_B200_NVFP4>(g, tm_a, tm_b, sms, st);
+    return format == GAT_B200_MXFP4 ? launch_product<GAT_B200_MXFP4>(g, a, lda, b, ldb, kb, sms, st)
+                                    : launch_product<GAT_B200_NVFP4>(g, a, lda, b, ldb, kb, sms, st);
 }
 
 int fp4_check_error() {

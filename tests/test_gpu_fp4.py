@@ -200,7 +200,7 @@ def check_product(got, a, b, bf16):
 PRODUCTS = [(1, 1, 1), (1, 16, 32), (1, 100, 64), (2, 129, 65), (3, 8, 33), (8, 512, 1024), (9, 300, 129), (16, 257, 4096),
             (17, 64, 300), (37, 203, 744), (64, 1000, 512), (65, 40, 200), (100, 128, 256), (128, 128, 256), (129, 130, 257),
             (200, 47, 256), (255, 256, 100), (256, 256, 512), (300, 384, 1111), (513, 200, 31), (1000, 700, 2000),
-            (4000, 256, 256), (3, 5003, 2744)]
+            (4000, 256, 256), (3, 5003, 2744), (4900, 1000, 300), (19000, 130, 520), (260, 18950, 77), (5001, 1025, 1500)]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -214,7 +214,8 @@ def test_product_matches_fp64(G, dev, fmt, bf16, m, n, k):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("m,n,ldo", [(5, 50, 53), (140, 99, 100), (300, 260, 264), (1, 33, 40)])
+@pytest.mark.parametrize("m,n,ldo", [(5, 50, 53), (140, 99, 100), (300, 260, 264), (1, 33, 40), (19001, 70, 71),
+                                      (18990, 100, 136)])
 def test_product_strides_leave_the_rest_alone(G, dev, fmt, m, n, ldo):
     k = 200
     a = table(features(m, k, 1, "f32"), fmt, dev, extra=32)
