@@ -247,54 +247,58 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc_s = idesc_bf16(kRows, kRows, 0, 0);
-            const uint32_t idesc_o = idesc_bf16(kRows, ksteps * 16, 0, 1);
-            bool ok = mbar_wait(q_full, 0, abort_flag, &g_attention_error);
-            uint32_t used[2] = {0, 0};  // blocks of tile t issued so far
-            auto scores = [&](int t, int j) {
-                const uint32_t qa = smem_u32(q_s + t * kTile), ka = smem_u32(k_s + (j % kSt) * kTile);
-                for (int ks = 0; ks < ksteps; ++ks) {
-                    const uint32_t off = (ks >> 2) * (kRows * 128) + (ks & 3) * 32;
-                    mma_bf16(tmem + 128 * t, desc_sw128(qa + off, 16, 1024), desc_sw128(ka + off, 16, 1024), idesc_s, ks > 0);
-                }
-                mma_commit(s_full + t);
-            };
-            for (int j = -1; j < blocks && ok; ++j) {
+        const uint32_t idesc_s = idesc_bf16(kRows, kRows, 0, 0);
+        const uint32_t idesc_o = idesc_bf16(kRows, ksteps * 16, 0, 1);
+        bool ok = mbar_wait_warp(q_full, 0, abort_flag, &g_attention_error);
+        uint32_t used[2] = {0, 0};  // blocks of tile t issued so far
+        for (int j = -1; j < blocks && ok; ++j) {
+            const int s = j % kSt, sn = (j + 1) % kSt;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (t > last_tile || !ok) break;
-                    if (j >= 0) {
-                        const int s = j % kSt;
-                        if (t == 0 && !mbar_wait(v_ready + s, uint32_t(j / kSt) & 1u, abort_flag, &g_attention_error)) { ok = false; break; }
-                        if (j >= from[t] && j < to[t]) {
-                            if (!mbar_wait(p_full + t, used[t] & 1u, abort_flag, &g_attention_error)) { ok = false; break; }
-                            ++used[t];
-                            fence_after();
-                            const uint32_t va = smem_u32(v_s + s * kTile);
+            for (int t = 0; t < 2; ++t) {
+                if (t > last_tile || !ok) break;
+                const bool now = j >= from[t] && j < to[t], next = j + 1 >= from[t] && j + 1 < to[t];
+                if (j >= 0) {
+                    if (t == 0) ok = mbar_wait_warp(v_ready + s, uint32_t(j / kSt) & 1u, abort_flag, &g_attention_error);
+                    if (ok && now) ok = mbar_wait_warp(p_full + t, used[t]++ & 1u, abort_flag, &g_attention_error);
+                    if (!ok) break;
+                    fence_after();
+                    const uint64_t vdesc = desc_sw128(smem_u32(v_s + s * kTile), kRows * 128, 1024);
+                    if (elect_one()) {
+                        if (now) {
 #pragma unroll
                             for (int ks = 0; ks < kRows / 16; ++ks)
-                                mma_bf16_ts(tmem + 256 + 128 * t, tmem + 128 * t + ks * 8,
-                                            desc_sw128(va + ks * 2048, kRows * 128, 1024), idesc_o);
+                                mma_bf16_ts(tmem + 256 + 128 * t, tmem + 128 * t + ks * 8, vdesc + ks * 128, idesc_o);
                             if (j + 1 == to[t]) mma_commit(o_full + t);
                         }
                         if (t == last_tile) mma_commit(v_empty + s);
                     }
-                    if (j + 1 < blocks) {
-                        const int s = (j + 1) % kSt;
-                        if (t == 0 && !mbar_wait(k_full + s, uint32_t((j + 1) / kSt) & 1u, abort_flag, &g_attention_error)) { ok = false; break; }
-                        if (j + 1 >= from[t] && j + 1 < to[t]) {
-                            fence_after();
-                            scores(t, j + 1);
+                    __syncwarp();
+                }
+                if (j + 1 < blocks) {
+                    if (t == 0) ok = mbar_wait_warp(k_full + sn, uint32_t((j + 1) / kSt) & 1u, abort_flag, &g_attention_error);
+                    if (!ok) break;
+                    fence_after();
+                    const uint64_t qdesc = desc_sw128(smem_u32(q_s + t * kTile), 16, 1024);
+                    const uint64_t kdesc = desc_sw128(smem_u32(k_s + sn * kTile), 16, 1024);
+                    if (elect_one()) {
+                        if (next) {
+#pragma unroll
+                            for (int ks = 0; ks < DP / 16; ++ks) {
+                                if (ks >= ksteps) break;
+                                const uint32_t off = (ks >> 2) * (kRows * 128 / 16) + (ks & 3) * 2;
+                                mma_bf16(tmem + 128 * t, qdesc + off, kdesc + off, idesc_s, ks > 0);
+                            }
+                            mma_commit(s_full + t);
                         }
-                        if (t == last_tile) mma_commit(k_empty + s);
+                        if (t == last_tile) mma_commit(k_empty + sn);
                     }
+                    __syncwarp();
                 }
             }
-            // whatever was issued has finished before the CTA ends (v_empty of the last block)
-            if (ok)
-                mbar_wait(v_empty + (blocks - 1) % kSt, uint32_t((blocks - 1) / kSt) & 1u, abort_flag, &g_attention_error);
         }
+        // whatever was issued has finished before the CTA ends (v_empty of the last block)
+        if (ok)
+            mbar_wait_warp(v_empty + (blocks - 1) % kSt, uint32_t((blocks - 1) / kSt) & 1u, abort_flag, &g_attention_error);
     } else if (warp < 4) {
         // ---- V of masked blocks: non-finite values out, their keys noted ----
         for (int j = 0; j < blocks; ++j) {

@@ -186,42 +186,46 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
                 mbar_wait(empty + i % kPairStages, (i / kPairStages) & 1u, abort_flag, &g_fp4_error);
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             uint32_t kc = 0, tl = 0;
             bool ok = true;
             const uint32_t sfa0 = tmem + kScaleCols, sfb0 = sfa0 + 4 * S::kTiles;
             for (uint32_t t = pair; t < ntiles && ok; t += pairs, ++tl) {
-                if (tl && !mbar_wait(drained, (tl - 1) & 1u, abort_flag, &g_fp4_error)) { ok = false; break; }
+                if (tl && !mbar_wait_warp(drained, (tl - 1) & 1u, abort_flag, &g_fp4_error)) { ok = false; break; }
                 fence_after();
                 const uint32_t d = tmem + ((tl & 1u) ? kOdd : 0);
                 for (int k = 0; k < g.stages_k; ++k, ++kc) {
                     const int s = int(kc % kPairStages);
-                    if (!mbar_wait(full + s, (kc / kPairStages) & 1u, abort_flag, &g_fp4_error)) { ok = false; break; }
+                    if (!mbar_wait_warp(full + s, (kc / kPairStages) & 1u, abort_flag, &g_fp4_error)) { ok = false; break; }
                     fence_after();
                     const uint32_t a_addr = smem_u32(smem + s * 2 * kHalf), b_addr = a_addr + kHalf;
-                    const uint32_t f = smem_u32(sf_s + s * 3 * S::kBytes);
+                    const uint64_t adesc = desc_sw128(a_addr, 16, 1024), bdesc = desc_sw128(b_addr, 16, 1024);
+                    const uint64_t fdesc = desc_scales(smem_u32(sf_s + s * 3 * S::kBytes));
                     const int mmas = k + 1 == g.stages_k ? g.last_mmas : 4;
+                    if (elect_one()) {
+                        // descriptors count in 16 bytes
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (j >= mmas) break;
-                        const int st = j / S::kTileMmas;
-                        const uint32_t sfa = sfa0 + st * 4, sfb = sfb0 + st * 8;
-                        if (j % S::kTileMmas == 0) {
-                            tmem_cp_scales<2>(sfa, desc_scales(f + st * 512));
-                            tmem_cp_scales<2>(sfb, desc_scales(f + S::kBytes + st * 512));
-                            tmem_cp_scales<2>(sfb + 4, desc_scales(f + 2 * S::kBytes + st * 512));
+                        for (int j = 0; j < 4; ++j) {
+                            if (j >= mmas) break;
+                            const int st = j / S::kTileMmas;
+                            const uint32_t sfa = sfa0 + st * 4, sfb = sfb0 + st * 8;
+                            if (j % S::kTileMmas == 0) {
+                                tmem_cp_scales<2>(sfa, fdesc + st * 32);
+                                tmem_cp_scales<2>(sfb, fdesc + S::kBytes / 16 + st * 32);
+                                tmem_cp_scales<2>(sfb + 4, fdesc + 2 * S::kBytes / 16 + st * 32);
+                            }
+                            mma_fp4<S::kMx, 2>(d, adesc + j * 2, bdesc + j * 2,
+                                               idesc_fp4(256, 256, S::kMx, S::kMx ? 2 * (j & 1) : 0), sfa, sfb,
+                                               (k | j) ? 1u : 0u);
                         }
-                        mma_fp4<S::kMx, 2>(d, desc_sw128(a_addr + j * 32, 16, 1024), desc_sw128(b_addr + j * 32, 16, 1024),
-                                           idesc_fp4(256, 256, S::kMx, S::kMx ? 2 * (j & 1) : 0), sfa, sfb,
-                                           (k | j) ? 1u : 0u);
+                        pair_commit(empty + s);
+                        if (k + 1 == g.stages_k) pair_commit(acc_full + (tl & 1u));
                     }
-                    pair_commit(empty + s);
+                    __syncwarp();
                 }
-                if (!ok) break;
-                pair_commit(acc_full + (tl & 1u));
             }
-            pair_commit(mma_done);
-            mbar_wait(mma_done, 0, abort_flag, &g_fp4_error);
+            if (elect_one()) pair_commit(mma_done);
+            mbar_wait_warp(mma_done, 0, abort_flag, &g_fp4_error);
         }
     } else {
         const int q = warp & 3, ew = warp - 2, set = ew >> 2;
@@ -407,33 +411,35 @@ __global__ void __launch_bounds__(kRowsThreads)
                 mbar_wait(full + i % kSt, (uint32_t(i) / kSt) & 1u, abort_flag, &g_fp4_error);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            // scales behind the accumulator; a's rows start a scale tile (below 128 rows there is one tile of them)
-            const uint32_t sfb0 = tmem + RowsTile<BN>::kCols, sfa0 = sfb0 + 4 * S::kTiles;
-            for (int k = k0; k < k1; ++k) {
-                const int i = k - k0, s = i % kSt;
-                if (!mbar_wait(full + s, (uint32_t(i) / kSt) & 1u, abort_flag, &g_fp4_error)) break;
-                fence_after();
-                const uint32_t b_addr = smem_u32(smem + s * kB), a_addr = smem_u32(a_s + s * kA);
-                const uint32_t f = smem_u32(sf_s + s * 2 * S::kBytes);
-                const int mmas = k + 1 == g.stages_k ? g.last_mmas : 4;
+        // scales behind the accumulator; a's rows start a scale tile (below 128 rows there is one tile of them)
+        const uint32_t sfb0 = tmem + RowsTile<BN>::kCols, sfa0 = sfb0 + 4 * S::kTiles;
+        for (int k = k0; k < k1; ++k) {
+            const int i = k - k0, s = i % kSt;
+            if (!mbar_wait_warp(full + s, (uint32_t(i) / kSt) & 1u, abort_flag, &g_fp4_error)) break;
+            fence_after();
+            const uint64_t adesc = desc_sw128(smem_u32(a_s + s * kA), 16, 1024);
+            const uint64_t bdesc = desc_sw128(smem_u32(smem + s * kB), 16, 1024);
+            const uint64_t fdesc = desc_scales(smem_u32(sf_s + s * 2 * S::kBytes));
+            const int mmas = k + 1 == g.stages_k ? g.last_mmas : 4;
+            if (elect_one()) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (j >= mmas) break;
                     const int st = j / S::kTileMmas;
                     if (j % S::kTileMmas == 0) {
-                        tmem_cp_scales<1>(sfb0 + st * 4, desc_scales(f + st * 512));
-                        tmem_cp_scales<1>(sfa0 + st * 4, desc_scales(f + S::kBytes + st * 512));
+                        tmem_cp_scales<1>(sfb0 + st * 4, fdesc + st * 32);
+                        tmem_cp_scales<1>(sfa0 + st * 4, fdesc + S::kBytes / 16 + st * 32);
                     }
-                    mma_fp4<S::kMx, 1>(tmem, desc_sw128(b_addr + j * 32, 16, 1024), desc_sw128(a_addr + j * 32, 16, 1024),
-                                       idesc_fp4(128, BN, S::kMx, S::kMx ? 2 * (j & 1) : 0), sfb0 + st * 4,
-                                       sfa0 + st * 4, (i | j) ? 1u : 0u);
+                    mma_fp4<S::kMx, 1>(tmem, bdesc + j * 2, adesc + j * 2,
+                                       idesc_fp4(128, BN, S::kMx, S::kMx ? 2 * (j & 1) : 0), sfb0 + st * 4, sfa0 + st * 4,
+                                       (i | j) ? 1u : 0u);
                 }
                 mma_commit(empty + s);
             }
-            mma_commit(acc_full);
-            mbar_wait(acc_full, 0, abort_flag, &g_fp4_error);
+            __syncwarp();
         }
+        if (elect_one()) mma_commit(acc_full);
+        mbar_wait_warp(acc_full, 0, abort_flag, &g_fp4_error);
     }
     // the accumulator is complete; nobody reads the stages any more
     bool ok = k1 > k0;
