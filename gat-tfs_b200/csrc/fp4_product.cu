@@ -67,9 +67,10 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t saddr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
     return r;
 }
+// Only tensor memory is handed over by it (tcgen05 fences order that), so it
+// needs no release at cluster scope, which waits for every store: 1100 cycles.
 __device__ __forceinline__ void mbar_arrive_rank(uint64_t* bar, uint32_t rank) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_to_rank(smem_u32(bar), rank))
-                 : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(map_to_rank(smem_u32(bar), rank)) : "memory");
 }
 // Loads of a CTA pair count on the first CTA's barrier (bit 24 of a shared
 // address holds the CTA's parity in the pair).
@@ -89,17 +90,18 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar) {
 }
 
 // ------------------------------------------------------------ CTA pairs
-// Roles of the 10 warps of each CTA of a pair:
+// Roles of the 20 warps of each CTA of a pair (2 and 3 idle):
 //   warp 0    TMA producer: this CTA's 128 rows of a, 128 of the tile's 256 rows
 //             of b (the pair's MMA reads both halves) and their scales; the
 //             scales of b's whole tile, which each CTA's tensor memory holds.
 //   warp 1    first CTA only: scale copies and MMAs of the pair.
-//   warps 2-9 epilogue of this CTA's 128 x 256 accumulators.
+//   warps 4-19 epilogue: 32 rows x 64 columns of this CTA's 128 x 256
+//             accumulators each, in registers at once, so the next tile's MMAs
+//             start while this one is scaled, rounded and stored.
 // Tensor memory: accumulators of even tiles in columns 0-255, of odd tiles in
-// 192-447, scales in 448-511. Two whole accumulators and the scales do not fit,
-// so they share 64 columns, which the epilogue drains first: the next tile's
-// MMAs start while three quarters of this one still leave.
-constexpr int kPairThreads = 320;
+// 192-447, scales in 448-511 (two whole accumulators and the scales do not fit).
+constexpr int kEpiWarps = 16;
+constexpr int kPairThreads = 128 + 32 * kEpiWarps;
 constexpr int kPairStages = 4;
 constexpr int kOdd = 192, kScaleCols = 448;
 
@@ -113,10 +115,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     constexpr int kStage = 2 * kHalf + 3 * S::kBytes;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* st_s = smem + kPairStages * 2 * kHalf;               // 8 warps x 2 x 4 KB
-    uint8_t* sf_s = st_s + 8 * 2 * 4096;                           // stages x 3 scale pieces
-    float* rb_s = reinterpret_cast<float*>(sf_s + kPairStages * 3 * S::kBytes);  // 8 warps x 64
-    uint64_t* bars = reinterpret_cast<uint64_t*>(rb_s + 8 * 64);
+    uint8_t* st_s = smem + kPairStages * 2 * kHalf;               // 4 KB per epilogue warp
+    uint8_t* sf_s = st_s + kEpiWarps * 4096;                       // stages x 3 scale pieces
+    float* rb_s = reinterpret_cast<float*>(sf_s + kPairStages * 3 * S::kBytes);  // 64 per epilogue warp
+    uint64_t* bars = reinterpret_cast<uint64_t*>(rb_s + kEpiWarps * 64);
     uint64_t* full = bars;
     uint64_t* empty = full + kPairStages;
     uint64_t* acc_full = empty + kPairStages;  // [2]
@@ -143,7 +145,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         }
         mbar_init(acc_full + 0, 1);
         mbar_init(acc_full + 1, 1);
-        mbar_init(drained, 16);
+        mbar_init(drained, 2 * kEpiWarps);
         mbar_init(mma_done, 1);
         *abort_flag = 0;
         fence_mbarrier_init();
@@ -227,97 +229,98 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             if (elect_one()) pair_commit(mma_done);
             mbar_wait_warp(mma_done, 0, abort_flag, &g_fp4_error);
         }
-    } else {
-        const int q = warp & 3, ew = warp - 2, set = ew >> 2;
-        uint8_t* stage = st_s + ew * 2 * 4096;
+    } else if (warp >= 4) {
+        const int q = warp & 3, ew = warp - 4, grp = ew >> 2;
+        uint8_t* sb = st_s + ew * 4096;
         float* rb = rb_s + ew * 64;
-        uint32_t tl = 0, toggle = 0;
-        for (uint32_t t = pair; t < ntiles; t += pairs, ++tl) {
-            uint32_t tm, tn;
+        // the row scales of a tile, fetched while the one before it is worked on
+        float ra = 1.f, rb0 = 0.f, rb1 = 0.f;
+        uint32_t tm = 0, tn = 0;
+        auto fetch = [&](uint32_t t) {
             tile_at(t, tm, tn);
+            const uint64_t r = uint64_t(tm) * 256 + rank * 128 + q * 32 + lane;
+            if (g.a_row && r < g.m) ra = g.a_row[r];
+            const int c = int(tn) * 256 + grp * 64 + lane;
+            if (g.b_row && c < g.n) rb0 = g.b_row[c];
+            if (g.b_row && c + 32 < g.n) rb1 = g.b_row[c + 32];
+        };
+        if (pair < ntiles) fetch(pair);
+        uint32_t tl = 0;
+        for (uint32_t t = pair; t < ntiles; t += pairs, ++tl) {
             const uint32_t odd = tl & 1u;
+            const uint64_t row0 = uint64_t(tm) * 256 + rank * 128 + q * 32;
+            const int col = int(tn) * 256 + grp * 64;
+            const float ra_t = ra;
+            __syncwarp();  // the last tile's reads of rb
+            rb[lane] = rb0;
+            rb[lane + 32] = rb1;
+            __syncwarp();
+            if (t + pairs < ntiles) fetch(t + pairs);
             if (!mbar_wait(acc_full + odd, (tl >> 1) & 1u, abort_flag, &g_fp4_error)) break;
             fence_after();
-            const uint32_t acc = tmem + (odd ? kOdd : 0) + (uint32_t(q * 32) << 16);
-            const uint64_t row0 = uint64_t(tm) * 256 + rank * 128 + q * 32;
-            const float ra = g.a_row && row0 + lane < g.m ? g.a_row[row0 + lane] : 1.f;
-#pragma unroll 1
-            for (int i = 0; i < 2; ++i) {
-                // 64-column groups in the order 3 2 | 1 0 (even tiles) and 0 1 | 2 3 (odd tiles) of the two sets
-                const int grp = odd ? 2 * set + i : 3 - 2 * set - i;
-                const int col = int(tn) * 256 + grp * 64;
-                if (g.b_row) {
-                    __syncwarp();
-                    rb[lane] = col + lane < g.n ? g.b_row[col + lane] : 0.f;
-                    rb[lane + 32] = col + lane + 32 < g.n ? g.b_row[col + lane + 32] : 0.f;
-                    __syncwarp();
-                }
-                float v[64];
-                tmem_ld64(acc + grp * 64, v);
-                // the shared columns are in registers (set 0), everything is (set 1)
-                if (i == set) {
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_rank(drained, 0);
-                }
-                if (col >= g.n || row0 >= g.m) continue;
-                if (g.b_row) {
+            float v[64];
+            tmem_ld64(tmem + (odd ? kOdd : 0) + (uint32_t(q * 32) << 16) + grp * 64, v);
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_rank(drained, 0);
+            if (col >= g.n || row0 >= g.m) continue;
+            if (g.b_row) {
 #pragma unroll
-                    for (int c = 0; c < 64; c += 4) {
-                        const float4 b4 = *reinterpret_cast<const float4*>(rb + c);
-                        v[c] *= ra * b4.x;
-                        v[c + 1] *= ra * b4.y;
-                        v[c + 2] *= ra * b4.z;
-                        v[c + 3] *= ra * b4.w;
+                for (int c = 0; c < 64; c += 4) {
+                    const float4 b4 = *reinterpret_cast<const float4*>(rb + c);
+                    v[c] *= ra_t * b4.x;
+                    v[c + 1] *= ra_t * b4.y;
+                    v[c + 2] *= ra_t * b4.z;
+                    v[c + 3] *= ra_t * b4.w;
+                }
+            } else if (g.a_row) {
+#pragma unroll
+                for (int c = 0; c < 64; ++c) v[c] *= ra_t;
+            }
+            // 32 rows x 128 bytes at a time, 16-byte pieces swizzled as the TMA store expects
+            auto stage = [&](int h, auto piece) {
+                const int c0 = col + h * 32, width = g.out_bf16 ? 64 : 32;
+                if (lane == 0) bulk_wait_read<0>();
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    *reinterpret_cast<uint4*>(sb + lane * 128 + ((c ^ (lane & 7)) * 16)) = piece(c);
+                // a TMA store writes whole 16-byte pieces: the last columns go out one by one unless n ends a piece
+                if (g.tma_out && (g.n_whole || c0 + width <= g.n)) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tm_out, sb, c0, int(row0));
+                        bulk_commit();
                     }
                 } else {
-#pragma unroll
-                    for (int c = 0; c < 64; ++c) v[c] *= ra;
+                    __syncwarp();
+                    for (int r = 0; r < 32 && row0 + r < g.m; ++r)
+                        for (int c = lane; c < width && c0 + c < g.n; c += 32) {
+                            const int byte = c * (g.out_bf16 ? 2 : 4);
+                            const uint8_t* src = sb + r * 128 + (((byte >> 4) ^ (r & 7)) * 16) + (byte & 15);
+                            const uint64_t off = (row0 + r) * uint64_t(g.ldo) + c0 + c;
+                            if (g.out_bf16)
+                                static_cast<uint16_t*>(g.out)[off] = *reinterpret_cast<const uint16_t*>(src);
+                            else
+                                static_cast<float*>(g.out)[off] = *reinterpret_cast<const float*>(src);
+                        }
+                    __syncwarp();
                 }
-                // 32 rows x 128 bytes at a time, 16-byte pieces swizzled as the TMA store expects
-                const int halves = g.out_bf16 ? 1 : 2;
+            };
+            if (g.out_bf16) {
+                stage(0, [&](int c) {
+                    return make_uint4(pack_bf16x2(v[8 * c], v[8 * c + 1]), pack_bf16x2(v[8 * c + 2], v[8 * c + 3]),
+                                      pack_bf16x2(v[8 * c + 4], v[8 * c + 5]), pack_bf16x2(v[8 * c + 6], v[8 * c + 7]));
+                });
+            } else {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    if (h >= halves || col + 32 * h >= g.n) break;
-                    uint8_t* sb = stage + toggle * 4096;
-                    toggle ^= 1u;
-                    if (lane == 0 && g.tma_out) bulk_wait_read<1>();
-                    __syncwarp();
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        uint4 w;
-                        if (g.out_bf16) {
-                            w = make_uint4(pack_bf16x2(v[8 * c], v[8 * c + 1]), pack_bf16x2(v[8 * c + 2], v[8 * c + 3]),
-                                           pack_bf16x2(v[8 * c + 4], v[8 * c + 5]), pack_bf16x2(v[8 * c + 6], v[8 * c + 7]));
-                        } else {
-                            w = make_uint4(__float_as_uint(v[32 * h + 4 * c]), __float_as_uint(v[32 * h + 4 * c + 1]),
-                                           __float_as_uint(v[32 * h + 4 * c + 2]), __float_as_uint(v[32 * h + 4 * c + 3]));
-                        }
-                        *reinterpret_cast<uint4*>(sb + lane * 128 + ((c ^ (lane & 7)) * 16)) = w;
-                    }
-                    // a TMA store writes whole 16-byte pieces: the last columns go out one by one unless n ends a piece
-                    if (g.tma_out && (g.n_whole || col + 32 * h + (g.out_bf16 ? 64 : 32) <= g.n)) {
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) {
-                            tma_store_2d(&tm_out, sb, col + 32 * h, int(row0));
-                            bulk_commit();
-                        }
-                    } else {
-                        if (lane == 0) bulk_commit();  // an empty group: the two buffers keep their turns
-                        __syncwarp();
-                        const int width = g.out_bf16 ? 64 : 32;
-                        for (int r = 0; r < 32 && row0 + r < g.m; ++r)
-                            for (int c = lane; c < width && col + 32 * h + c < g.n; c += 32) {
-                                const int byte = c * (g.out_bf16 ? 2 : 4);
-                                const uint8_t* src = sb + r * 128 + (((byte >> 4) ^ (r & 7)) * 16) + (byte & 15);
-                                const uint64_t off = (row0 + r) * uint64_t(g.ldo) + col + 32 * h + c;
-                                if (g.out_bf16)
-                                    static_cast<uint16_t*>(g.out)[off] = *reinterpret_cast<const uint16_t*>(src);
-                                else
-                                    static_cast<float*>(g.out)[off] = *reinterpret_cast<const float*>(src);
-                            }
-                    }
+                    if (col + 32 * h >= g.n) break;
+                    stage(h, [&](int c) {
+                        return make_uint4(__float_as_uint(v[32 * h + 4 * c]), __float_as_uint(v[32 * h + 4 * c + 1]),
+                                          __float_as_uint(v[32 * h + 4 * c + 2]), __float_as_uint(v[32 * h + 4 * c + 3]));
+                    });
                 }
             }
         }
@@ -539,7 +542,7 @@ int launch_pair(ProductArgs g, const void* a, int lda, const void* b, int ldb, i
     } else {
         tm_out = tm_a;  // not used
     }
-    constexpr int smem = kPairStages * (2 * 16384 + 3 * S::kBytes) + 8 * 2 * 4096 + 8 * 64 * 4 + 256 + 1024;
+    constexpr int smem = kPairStages * (2 * 16384 + 3 * S::kBytes) + kEpiWarps * (4096 + 256) + 256 + 1024;
     auto kern = pair_kernel<FORMAT>;
     GATB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     const uint64_t ntiles = uint64_t(g.grid_m) * g.grid_n;
