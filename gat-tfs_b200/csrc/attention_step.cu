@@ -3,9 +3,11 @@
 // The bytes of K and V bound it: every key and value is read once, for all
 // query heads of its key head together (up to eight a CTA). The keys of all
 // segments, laid end to end, are cut into equal runs, one per CTA column, so
-// neither one long segment nor many ragged ones leave SMs idle; a segment cut
-// by a run's border leaves a partial state (maximum, sum, weighted values) per
-// piece, and a second kernel joins a segment's pieces in their order.
+// neither one long segment nor many ragged ones leave SMs idle (each segment
+// counts as kPieceCost keys more than it has: what starting a piece costs). A
+// segment cut by a run's border leaves a partial state (maximum, sum, weighted
+// values) per piece, and a second kernel, started ahead by programmatic launch,
+// joins a segment's pieces in their order.
 //
 // A warp takes 32 keys at a time, straight from global memory into the
 // fragments of mma.sync m16n8k16 (16-byte loads; which of the 16 reduction
@@ -21,6 +23,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kKeys = 32;       // keys of a warp's step
 constexpr int kHeadTile = 8;    // query heads of a CTA
+constexpr uint64_t kPieceCost = kWarps * kKeys;
 
 struct StepArgs {
     uint64_t n_k;
@@ -45,12 +48,15 @@ __device__ __forceinline__ uint64_t seg_len(const StepArgs& a, int s) {
     return b >= a.n_k ? 0 : min(l, a.n_k - b);
 }
 
-// Keys of all segments and keys before segment `upto`; all threads of the CTA.
+// Places of a segment in the runs.
+__device__ __forceinline__ uint64_t seg_places(uint64_t len) { return len ? len + kPieceCost : 0; }
+
+// Places of all segments and places before segment `upto`; all threads of the CTA.
 __device__ __forceinline__ void count_keys(const StepArgs& a, int upto, uint64_t& total, uint64_t& before) {
     __shared__ uint64_t part[2][32];
     uint64_t t = 0, b = 0;
     for (int s = threadIdx.x; s < a.nseg; s += blockDim.x) {
-        const uint64_t l = seg_len(a, s);
+        const uint64_t l = seg_places(seg_len(a, s));
         t += l;
         if (s < upto) b += l;
     }
@@ -71,8 +77,8 @@ __device__ __forceinline__ void count_keys(const StepArgs& a, int upto, uint64_t
     }
     __syncthreads();
 }
-// Keys of a run: the total in `runs` parts, whole steps of a CTA.
-__device__ __forceinline__ uint64_t run_keys(uint64_t total, int runs) {
+// Places of a run: the total in `runs` parts, whole steps of a CTA.
+__device__ __forceinline__ uint64_t run_places(uint64_t total, int runs) {
     constexpr uint64_t unit = kWarps * kKeys;
     const uint64_t c = (total + runs - 1) / runs;
     return (c + unit - 1) / unit * unit;
@@ -104,14 +110,23 @@ __global__ void __launch_bounds__(kWarps * 32) attention_step_kernel(const StepA
     const int kvh = blockIdx.y, head0 = kvh * a.group + blockIdx.z * kHeadTile;
     const int live_heads = min(kHeadTile, a.group - int(blockIdx.z) * kHeadTile);
 
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (a.runs == 1) {  // no second kernel: segments without keys are written here
+        for (int s = 0; s < a.nseg; ++s) {
+            if (seg_len(a, s)) continue;
+            for (int e = threadIdx.x; e < live_heads * a.dim; e += kWarps * 32)
+                a.out[uint64_t(s) * a.ldo + uint64_t(head0) * a.dim + e] = 0;
+            if (a.lse && int(threadIdx.x) < live_heads) a.lse[uint64_t(s) * a.heads + head0 + threadIdx.x] = -INFINITY;
+        }
+    }
     uint64_t total, unused;
     count_keys(a, 0, total, unused);
-    const uint64_t run = run_keys(total, a.runs);
+    const uint64_t run = run_places(total, a.runs);
     const uint64_t v0 = run * blockIdx.x, v1 = min(total, v0 + run);
     if (v0 >= v1) return;
     // first segment that reaches past v0
     int seg = 0;
-    uint64_t seg_start = 0;  // keys before it
+    uint64_t seg_start = 0;  // places before it
     {
         __shared__ uint64_t sums[kWarps];
         __shared__ int found;
@@ -120,7 +135,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_step_kernel(const StepA
         __syncthreads();
         for (int base = 0; base < a.nseg; base += kWarps * 32) {
             const int s = base + threadIdx.x;
-            const uint64_t l = s < a.nseg ? seg_len(a, s) : 0;
+            const uint64_t l = s < a.nseg ? seg_places(seg_len(a, s)) : 0;
             uint64_t inc = l;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -157,7 +172,11 @@ __global__ void __launch_bounds__(kWarps * 32) attention_step_kernel(const StepA
         if (len == 0) continue;
         const uint64_t j0 = at - seg_start, j1 = min(len, v1 - seg_start);
         const bool entire = j0 == 0 && j1 == len;
-        at = seg_start + j1;
+        at = seg_start + seg_places(len);
+        if (j0 >= j1) {  // only the places behind its keys
+            seg_start = at;
+            continue;
+        }
         const uint64_t kbase = a.begin[seg];
         // Q as B fragments: head rr, the 8 columns 32 i + 8 qq of two reduction steps
         uint4 qf[2 * SETS];
@@ -315,50 +334,77 @@ __global__ void __launch_bounds__(kWarps * 32) attention_step_kernel(const StepA
             }
         }
         __syncthreads();
-        seg_start += len;
+        seg_start = at;
     }
 }
 
+constexpr int kMostRuns = 512;  // runs are never more than this
+constexpr int kJoinGroups = 4;  // groups of 128 threads, a column each, share the pieces
+
 // Grid (segments, heads): joins the pieces of a segment that runs cut, writes
 // zeros for a segment without keys.
-__global__ void __launch_bounds__(128) attention_join_kernel(const StepArgs a) {
-    const int seg = blockIdx.x, head = blockIdx.y, c = threadIdx.x;
+__global__ void __launch_bounds__(kJoinGroups * 128) attention_join_kernel(const StepArgs a) {
+    __shared__ float f_s[kMostRuns], red[kJoinGroups * 4], acc_s[kJoinGroups][128];
+    const int seg = blockIdx.x, head = blockIdx.y, c = threadIdx.x & 127, grp = threadIdx.x >> 7;
     uint64_t total, start;
     count_keys(a, seg, total, start);
     const uint64_t len = seg_len(a, seg);
     uint16_t* out = a.out + uint64_t(seg) * a.ldo + uint64_t(head) * a.dim;
+    const uint64_t run = run_places(total, a.runs);
+    const uint64_t first = len ? start / run : 0, last = len ? (start + len - 1) / run : 0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the pieces are written
     if (len == 0) {
-        if (c < a.dim) out[c] = 0;
-        if (c == 0 && a.lse) a.lse[uint64_t(seg) * a.heads + head] = -INFINITY;
+        if (threadIdx.x < unsigned(a.dim)) out[c] = 0;
+        if (threadIdx.x == 0 && a.lse) a.lse[uint64_t(seg) * a.heads + head] = -INFINITY;
         return;
     }
-    const uint64_t run = run_keys(total, a.runs);
-    const uint64_t first = start / run, last = (start + len - 1) / run;
     if (first == last) return;  // one piece: written already
     const uint64_t stride = uint64_t(a.heads) * (a.dim + 2);
     const float* p = a.part + ((first + seg) * a.heads + head) * uint64_t(a.dim + 2);
     const int n = int(last - first + 1);
-    float mm = -INFINITY;
-    for (int i = 0; i < n; ++i) mm = fmaxf(mm, p[i * stride + a.dim]);
-    const float ref = mm == -INFINITY ? 0.f : mm;
-    float sum = 0.f, acc = 0.f;
-    for (int i = 0; i < n; ++i) {
-        const float f = ex2(p[i * stride + a.dim] - ref);
-        sum = fmaf(p[i * stride + a.dim + 1], f, sum);
-        if (c < a.dim) acc = fmaf(p[i * stride + c], f, acc);
+    // thread i: piece i's maximum and sum
+    const bool mine = int(threadIdx.x) < n;
+    const float m = mine ? p[threadIdx.x * stride + a.dim] : -INFINITY;
+    const float l = mine ? p[threadIdx.x * stride + a.dim + 1] : 0.f;
+    float mm = warp_max(m);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mm;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJoinGroups * 4; ++w) mm = fmaxf(mm, red[w]);
+    __syncthreads();
+    const float f = ex2(m - (mm == -INFINITY ? 0.f : mm));
+    if (mine) f_s[threadIdx.x] = f;
+    const float part = warp_sum(mine ? l * f : 0.f);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = part;
+    __syncthreads();
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinGroups * 4; ++w) sum += red[w];
+    float acc = 0.f;
+    if (c < a.dim) {
+#pragma unroll 8
+        for (int i = grp; i < n; i += kJoinGroups) acc = fmaf(p[i * stride + c], f_s[i], acc);
     }
-    if (c < a.dim) out[c] = uint16_t(pack_bf16x2(acc / sum, 0.f));
-    if (c == 0 && a.lse) a.lse[uint64_t(seg) * a.heads + head] = (mm + log2f(sum)) * kLn2;
+    acc_s[grp][c] = acc;
+    __syncthreads();
+    if (threadIdx.x < unsigned(a.dim)) {
+        acc = acc_s[0][c];
+#pragma unroll
+        for (int g = 1; g < kJoinGroups; ++g) acc += acc_s[g][c];
+        out[c] = uint16_t(pack_bf16x2(acc / sum, 0.f));
+    }
+    if (threadIdx.x == 0 && a.lse) a.lse[uint64_t(seg) * a.heads + head] = (mm + log2f(sum)) * kLn2;
 }
 
-// Runs the keys are cut into: enough CTAs for `sms` SMs, no more than there can be keys for.
-int step_runs(int kv_heads, int group, uint64_t n_k, int nseg, int sms) {
+// Runs the keys are cut into: all the CTAs that fit the SMs at once (three or
+// two an SM by their registers), no more than there can be keys for.
+int step_runs(int kv_heads, int group, int dim, uint64_t n_k, int sms) {
     const int columns = kv_heads * ((group + kHeadTile - 1) / kHeadTile);
-    const uint64_t want = uint64_t((2 * sms + columns - 1) / columns);
-    const uint64_t most = (n_k + kWarps * kKeys - 1) / (kWarps * kKeys) + uint64_t(nseg);
-    return int(want < most ? want : most);
+    const uint64_t want = uint64_t((dim <= 64 ? 3 : 2) * sms / columns);
+    const uint64_t most = (n_k + kWarps * kKeys - 1) / (kWarps * kKeys);
+    const uint64_t runs = want < most ? want : most;
+    return runs < 1 ? 1 : runs > uint64_t(kMostRuns) ? kMostRuns : int(runs);
 }
-constexpr int kMostRuns = 512;  // runs are never more than this
 
 }  // namespace
 
@@ -396,8 +442,7 @@ int masked_attention_step_launch(const AttentionShape& s, int nseg, uint64_t n_k
     a.group = s.heads / s.kv_heads;
     a.dim = s.dim;
     a.nseg = nseg;
-    a.runs = step_runs(a.kv_heads, a.group, n_k, nseg, sms);
-    a.runs = a.runs > kMostRuns ? kMostRuns : (a.runs < 1 ? 1 : a.runs);
+    a.runs = step_runs(a.kv_heads, a.group, a.dim, n_k, sms);
     a.begin = begin;
     a.length = length;
     a.slopes = s.slopes;
@@ -428,8 +473,17 @@ int masked_attention_step_launch(const AttentionShape& s, int nseg, uint64_t n_k
         else go(attention_step_kernel<2, false, false>);
     }
     GATB_LAUNCH("masked_attention_step kernel");
-    attention_join_kernel<<<dim3(unsigned(nseg), unsigned(s.heads)), 128, 0, st>>>(a);
-    GATB_LAUNCH("masked_attention_step join kernel");
+    if (a.runs == 1) return 0;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(nseg), unsigned(s.heads));
+    cfg.blockDim = dim3(kJoinGroups * 128);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    GATB_CUDA(cudaLaunchKernelEx(&cfg, attention_join_kernel, a));
     return 0;
 }
 

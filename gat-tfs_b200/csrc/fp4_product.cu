@@ -345,7 +345,7 @@ constexpr int kRowsThreads = 192;
 
 template <int BN>
 struct RowsTile {
-    static constexpr int kStages = 4;
+    static constexpr int kStages = BN <= 16 ? 5 : 4;  // two CTAs an SM up to 32 rows
     static constexpr int kCols = BN <= 16 ? 32 : BN;  // accumulator columns, up to 32 of scales behind them
     static constexpr int kTmem = BN <= 32 ? 64 : (BN <= 64 ? 128 : 256);
 };
@@ -367,7 +367,8 @@ __global__ void __launch_bounds__(kRowsThreads)
     uint64_t* full = bars;
     uint64_t* empty = full + kSt;
     uint64_t* acc_full = empty + kSt;
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_full + 1);
+    float* ra_s = reinterpret_cast<float*>(acc_full + 1);  // [BN] row scales of a
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(ra_s + BN);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
     float* part = reinterpret_cast<float*>(smem);  // [BN][kPitch], over the stages once they are used up
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -375,7 +376,21 @@ __global__ void __launch_bounds__(kRowsThreads)
     const uint32_t tile = blockIdx.x / split;
     const uint32_t tn = tile % g.grid_n, tm = tile / g.grid_n;  // 128 rows of b, BN rows of a
     const int k0 = int(uint64_t(g.stages_k) * rank / split), k1 = int(uint64_t(g.stages_k) * (rank + 1) / split);
+    const uint64_t arow = uint64_t(tm) * BN;
+    auto load = [&](int k) {
+        const int s = (k - k0) % kSt;
+        const int sft = min(S::kTiles, g.tiles - k * S::kTiles);
+        mbar_expect_tx(full + s, kB + kA + 2 * 512 * sft);
+        tma_load_2d(smem + s * kB, &tm_b, full + s, k * 128, int(tn * 128));
+        tma_load_2d(a_s + s * kA, &tm_a, full + s, k * 128, int(arow));
+        uint8_t* f = sf_s + s * 2 * S::kBytes;
+        bulk_load(f, g.b_scales + (uint64_t(tn) * g.tiles + k * S::kTiles) * 512, 512 * sft, full + s);
+        bulk_load(f + S::kBytes, g.a_scales + ((arow >> 7) * uint64_t(g.tiles) + k * S::kTiles) * 512, 512 * sft, full + s);
+    };
 
+    float rb = 1.f;
+    const int q = warp & 3;
+    const int col = int(tn) * 128 + q * 32 + lane;  // output column: a row of b
     if (threadIdx.x == 0) {
         for (int s = 0; s < kSt; ++s) {
             mbar_init(full + s, 1);
@@ -384,11 +399,17 @@ __global__ void __launch_bounds__(kRowsThreads)
         mbar_init(acc_full, 1);
         *abort_flag = 0;
         fence_mbarrier_init();
-    }
-    if (warp == 1) {
+        // the first stages are on their way while the CTA sets itself up
+        for (int k = k0; k < min(k1, k0 + kSt); ++k) load(k);
+    } else if (warp == 1) {
+        __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
                      "r"(kTmem));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else if (warp >= 2) {
+        if (g.b_row && col < g.n) rb = g.b_row[col];
+        if (g.a_row)
+            for (int r = threadIdx.x - 64; r < BN; r += 128) ra_s[r] = arow + r < g.m ? g.a_row[arow + r] : 0.f;
     }
     fence_before();
     __syncthreads();
@@ -397,18 +418,11 @@ __global__ void __launch_bounds__(kRowsThreads)
 
     if (warp == 0) {
         if (lane == 0) {
-            const uint64_t arow = uint64_t(tm) * BN;
-            int k = k0;
+            int k = min(k1, k0 + kSt);
             for (; k < k1; ++k) {
-                const int i = k - k0, s = i % kSt;
-                if (!mbar_wait(empty + s, ((uint32_t(i) / kSt) & 1u) ^ 1u, abort_flag, &g_fp4_error)) break;
-                const int sft = min(S::kTiles, g.tiles - k * S::kTiles);
-                mbar_expect_tx(full + s, kB + kA + 2 * 512 * sft);
-                tma_load_2d(smem + s * kB, &tm_b, full + s, k * 128, int(tn * 128));
-                tma_load_2d(a_s + s * kA, &tm_a, full + s, k * 128, int(arow));
-                uint8_t* f = sf_s + s * 2 * S::kBytes;
-                bulk_load(f, g.b_scales + (uint64_t(tn) * g.tiles + k * S::kTiles) * 512, 512 * sft, full + s);
-                bulk_load(f + S::kBytes, g.a_scales + ((arow >> 7) * uint64_t(g.tiles) + k * S::kTiles) * 512, 512 * sft, full + s);
+                const int i = k - k0;
+                if (!mbar_wait(empty + i % kSt, ((uint32_t(i) / kSt) & 1u) ^ 1u, abort_flag, &g_fp4_error)) break;
+                load(k);
             }
             for (int i = max(0, k - k0 - kSt); i < k - k0; ++i)
                 mbar_wait(full + i % kSt, (uint32_t(i) / kSt) & 1u, abort_flag, &g_fp4_error);
@@ -448,11 +462,10 @@ __global__ void __launch_bounds__(kRowsThreads)
     bool ok = k1 > k0;
     if (warp >= 2 && ok) ok = mbar_wait(acc_full, 0, abort_flag, &g_fp4_error);
     __syncthreads();
-    const int q = warp & 3;
-    const int col = int(tn) * 128 + q * 32 + lane;  // output column: a row of b
-    const uint64_t arow = uint64_t(tm) * BN;
     const int rows = int(min(uint64_t(BN), g.m - arow));
     auto store = [&](int r, float y) {
+        if (col >= g.n) return;
+        y *= g.a_row ? rb * ra_s[r] : rb;
         const uint64_t off = (arow + r) * uint64_t(g.ldo) + col;
         if (g.out_bf16)
             static_cast<uint16_t*>(g.out)[off] = uint16_t(pack_bf16x2(y, 0.f));
@@ -461,19 +474,17 @@ __global__ void __launch_bounds__(kRowsThreads)
     };
     if (warp >= 2) {
         fence_after();
-        const float rb = g.b_row && col < g.n ? g.b_row[col] : 1.f;
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 16) {
-            if (c >= rows) break;
+        for (int c = 0; c < rows; c += 16) {
             float v[16];
             tmem_ld16(tmem + (uint32_t(q * 32) << 16) + c, v);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float y = ok ? v[i] : 0.f;  // a CTA without columns of the reduction adds nothing
+                const float y = ok ? v[i] : 0.f;  // a CTA that gave up adds nothing
                 if (split > 1)
                     part[(c + i) * kPitch + q * 32 + lane] = y;
-                else if (c + i < rows && col < g.n)
-                    store(c + i, g.a_row ? y * (rb * g.a_row[arow + c + i]) : y * rb);
+                else if (c + i < rows)
+                    store(c + i, y);
             }
         }
         fence_before();
@@ -481,16 +492,22 @@ __global__ void __launch_bounds__(kRowsThreads)
     if (split > 1) {
         cluster_sync();
         if (warp >= 2) {
-            const float rb = g.b_row && col < g.n ? g.b_row[col] : 1.f;
-            for (int r = int(rank); r < rows; r += split) {
-                const uint32_t at = smem_u32(part + r * kPitch + q * 32 + lane);
-                float y = 0.f;
+            // rows rank, rank + split, ...: four rows' loads from the cluster in flight at a time
+            for (int r0 = int(rank); r0 < rows; r0 += 4 * split) {
+                float y[4] = {0.f, 0.f, 0.f, 0.f};
                 for (int c = 0; c < split; ++c) {
-                    float x;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(map_to_rank(at, uint32_t(c))));
-                    y += x;
+                    const uint32_t base = map_to_rank(smem_u32(part), uint32_t(c));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = min(r0 + i * split, BN - 1);
+                        float x;
+                        asm("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(base + (r * kPitch + q * 32 + lane) * 4) : "memory");
+                        y[i] += x;
+                    }
                 }
-                if (col < g.n) store(r, g.a_row ? y * (rb * g.a_row[arow + r]) : y * rb);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (r0 + i * split < rows) store(r0 + i * split, y[i]);
             }
         }
         cluster_sync();  // the others have read this CTA's part
@@ -567,7 +584,7 @@ int launch_rows(ProductArgs g, const void* a, int lda, const void* b, int ldb, i
     constexpr int stages = RowsTile<BN>::kStages * (128 * 128 + BN * 128 + 2 * S::kBytes);
     constexpr int part = BN * 132 * 4;
     static_assert(part <= stages, "the exchange buffer lies over the stages");
-    constexpr int smem = stages + 256 + 1024;
+    constexpr int smem = stages + 256 + BN * 4 + 1024;
     auto kern = rows_kernel<FORMAT, BN>;
     GATB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg{};
