@@ -7,21 +7,25 @@
 // so a tile of 128 packed rows may span many segments: small graphs share tiles
 // and a long document is one run of tiles.
 //
-// One CTA: two tiles of 128 rows of one head, all key blocks of 128 that one of
-// their rows sees. 12 warps:
-//   warp 0     TMA producer: Q once, K and V blocks through rings.
-//   warp 1     MMA issuer: S = Q K^T into TMEM; O += P V with P read from TMEM
-//              (P overlays S). The tiles alternate, so one tile's softmax runs
-//              beside the other's MMAs.
-//   warps 2-3  masked blocks only: take non-finite values of V out of shared
-//              memory (a weight of zero times Inf or NaN is NaN) and note their
-//              keys; rows that do see such a key add it themselves.
-//   warps 4-7 / 8-11  softmax of tile 0 / 1, a row per thread: no shuffles.
+// One CTA: TILES tiles of 128 rows of one head, all key blocks of 128 that one
+// of their rows sees. Up to dim 64 a CTA has one tile and two CTAs share an SM;
+// above, shared memory holds one CTA and it has two tiles. Either way one
+// tile's softmax runs beside the other's MMAs. Warps:
+//   0     TMA producer: Q once, K and V blocks through rings.
+//   1     MMA issuer: S = Q K^T into TMEM; O += P V with P read from TMEM (P
+//         overlays S).
+//   2-3   masked blocks only: take non-finite values of V out of shared memory
+//         (a weight of zero times Inf or NaN is NaN) and note their keys; rows
+//         that do see such a key add it themselves.
+//   4 ..  softmax, four warps a tile, a row per thread: no shuffles.
 // The running maximum is only moved when it grows by more than 8 (a factor of
 // 256 in the weights, far inside FP32 and BF16's range), so O is seldom rescaled.
 // MMAs of a CTA run in order, so S's barrier also says that the tile's last P V
 // is done and O is at rest. P is rounded to BF16 (the tensor cores' input type;
 // the sum keeps the unrounded FP32 weights).
+// The exponentials bound it (16 a clock and SM; a 128 x 128 block of dim 128
+// takes the tensor cores as long as its exponentials): the cap's tanh is a
+// polynomial on the FMA pipe wherever a block's scores stay below 0.6 cap.
 #include <cuda.h>
 
 #include "attention.cuh"
@@ -39,7 +43,6 @@ namespace {
 using namespace tc;
 
 constexpr int kRows = 128;  // rows of a tile, keys of a block
-constexpr int kThreads = 384;
 
 struct AttnArgs {
     uint64_t n_q, n_k;
@@ -52,12 +55,14 @@ struct AttnArgs {
     int ldv;
     float zscale;    // without a cap: scale * log2 e; with one: 2 log2 e * scale / cap
     float zcap;      // cap * log2 e
+    float tscale;    // scale / cap
+    float small;     // raw scores up to which the tanh's polynomial holds
+    float tanh[5];   // its coefficients times zcap
     uint16_t* out;
     int ldo;
     float* lse;
 };
 
-// TMEM: S / P of tile t at 128 t, O of tile t at 256 + 128 t.
 __device__ __forceinline__ void mma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc) {
     asm volatile("tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, 1;" ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc),
                  "r"(idesc)
@@ -82,30 +87,87 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
         : "memory");
 }
 
-// Largest s with row[s] <= i, of nseg + 1 ascending row pointers.
-__device__ __forceinline__ int segment_of(const uint64_t* row, int nseg, uint64_t i) {
+// Segments of the 32 consecutive rows first + lane (a converged warp): the
+// first row's by a 32-way search, the others' from the row pointers behind it.
+__device__ __forceinline__ int segment_of_lane(const uint64_t* row, int nseg, uint64_t first, int lane) {
     int a = 0, b = nseg;
     while (b - a > 1) {
-        const int mid = (a + b) >> 1;
-        if (row[mid] <= i)
-            a = mid;
-        else
-            b = mid;
+        const int step = (b - a + 31) / 32, at = a + lane * step;
+        const unsigned le = __ballot_sync(0xffffffffu, at < b && row[at] <= first);
+        const int n = max(1, __popc(le));
+        a += (n - 1) * step;
+        b = min(b, a + step);
     }
-    return a;
+    int s = a;
+    for (int next = a + 1; next < nseg; next += 32) {
+        // rows at and past o belong to segment next + lane or a later one
+        const int at = next + lane;
+        const int o = at < nseg ? int(min(uint64_t(32), row[at] > first ? row[at] - first : 0)) : 32;
+        const unsigned live = __ballot_sync(0xffffffffu, o < 32);
+        for (int l = 0; l < __popc(live); ++l)
+            if (__shfl_sync(0xffffffffu, o, l) <= lane) ++s;
+        if (live != 0xffffffffu) break;
+    }
+    return min(s, nseg - 1);
 }
 
+// Two FP32 operations in one instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float x, float y) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& x, float& y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// tanh(x) = x p(x^2) for |x| <= 0.6, relative error 7.4e-8 (minimax, Remez exchange).
+constexpr float kTanhLimit = 0.6f;
+constexpr float kTanh[5] = {0.999999926872f, -0.333323099889f, 0.133101737673f, -0.0521014822761f, 0.0154754278422f};
+
 // DP: dim rounded up to 64 or 128. CAP / BIAS: scores go through the tanh / get the distance bias.
+// TMEM: S / P of tile t at 128 t, O of tile t at 128 TILES + DP t.
+template <int DP>
+struct Shape {
+    static constexpr int kTiles = DP == 64 ? 1 : 2;
+    static constexpr int kThreads = 128 + 128 * kTiles;
+    static constexpr int kCtas = DP == 64 ? 2 : 1;       // per SM
+    static constexpr int kTmem = DP == 64 ? 256 : 512;
+    static constexpr int kTile = kRows * DP * 2;         // bytes of a Q tile, a K block, a V block
+    static constexpr int kStages = 2;                    // K and V stages
+    static constexpr int kSmem = (kTiles + 2 * kStages) * kTile + 1024 + 512;
+};
 template <int DP, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
     attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnArgs g) {
-    constexpr int kTile = kRows * DP * 2;  // bytes of a Q tile, a K block, a V block
-    constexpr int kSt = DP == 64 ? 4 : 2;  // K and V stages
+    constexpr int kTiles = Shape<DP>::kTiles, kTile = Shape<DP>::kTile, kSt = Shape<DP>::kStages;
+    constexpr uint32_t kO = 128 * kTiles;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* q_s = smem;
-    uint8_t* k_s = q_s + 2 * kTile;
+    uint8_t* k_s = q_s + kTiles * kTile;
     uint8_t* v_s = k_s + kSt * kTile;
     uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + kSt * kTile);
     uint64_t* q_full = bars;
@@ -114,17 +176,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* v_full = k_empty + kSt;
     uint64_t* v_ready = v_full + kSt;
     uint64_t* v_empty = v_ready + kSt;
-    uint64_t* s_full = v_empty + kSt;  // [2]
-    uint64_t* p_full = s_full + 2;     // [2]
-    uint64_t* o_full = p_full + 2;     // [2]
-    uint32_t* bad = reinterpret_cast<uint32_t*>(o_full + 2);  // [kSt][4] keys of the block with non-finite values
+    uint64_t* s_full = v_empty + kSt;    // [kTiles]
+    uint64_t* p_full = s_full + kTiles;  // [kTiles]
+    uint64_t* o_full = p_full + kTiles;  // [kTiles]
+    uint32_t* bad = reinterpret_cast<uint32_t*>(o_full + kTiles);  // [kSt][4] keys of the block with non-finite values
     unsigned* range = bad + 4 * kSt;  // per tile: smallest lo, largest hi, largest lo, smallest hi
-    uint32_t* tmem_holder = range + 8;
+    uint32_t* tmem_holder = range + 4 * kTiles;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int head = int(blockIdx.x % unsigned(g.heads)), kv_head = head / g.group;
     // later rows see more keys under a causal mask: the longest tiles of all heads start first
-    const uint64_t row0 = uint64_t((gridDim.x - 1 - blockIdx.x) / unsigned(g.heads)) * (2 * kRows);
+    const uint64_t row0 = uint64_t((gridDim.x - 1 - blockIdx.x) / unsigned(g.heads)) * (kTiles * kRows);
+    const int boxes = g.dim > 64 ? 2 : 1;
+    const uint32_t bytes = uint32_t(boxes) * kRows * 128;  // of a tile or block as TMA counts them
+    const int q_tiles = row0 + kRows < g.n_q ? kTiles : 1;
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
@@ -135,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(v_ready + s, 2);
             mbar_init(v_empty + s, 1);
         }
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < kTiles; ++t) {
             mbar_init(s_full + t, 1);
             mbar_init(p_full + t, 4);
             mbar_init(o_full + t, 1);
@@ -146,16 +211,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         *abort_flag = 0;
         fence_mbarrier_init();
+        mbar_expect_tx(q_full, bytes * q_tiles);
+        for (int t = 0; t < q_tiles; ++t)
+            for (int b = 0; b < boxes; ++b)
+                tma_load_3d(q_s + t * kTile + b * (kRows * 128), &tm_q, q_full, b * 64, head, int(row0) + t * kRows);
     }
     if (warp == 1) {
+        __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
-                     "r"(512));
+                     "r"(Shape<DP>::kTmem));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    fence_before();
-    __syncthreads();
-    fence_after();
-    const uint32_t tmem = *tmem_holder;
 
     // The row's key interval (softmax threads), its position and the tile's ranges.
     const int tile = warp >= 8 ? 1 : 0;
@@ -163,13 +229,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t row = row0 + uint64_t(tile) * kRows + r;
     int lo = 0, hi = 0, pos = 0;
     if (warp >= 4) {
-        const bool live = row < g.n_q;
-        if (live) {
-            const int s = segment_of(g.q_row, g.nseg, row);
+        const int s = segment_of_lane(g.q_row, g.nseg, row - lane, lane);
+        if (row < g.n_q) {
             // row pointers are taken as given but kept inside the tables
+            const uint64_t q0 = g.q_row[s], q1 = g.q_row[s + 1];
             const uint64_t ks = min(g.k_row[s], g.n_k), ke = max(ks, min(g.k_row[s + 1], g.n_k));
-            const int64_t at = int64_t(row - min(g.q_row[s], row)) + int64_t(ke - ks) -
-                               int64_t(max(g.q_row[s + 1], g.q_row[s]) - g.q_row[s]);
+            const int64_t at = int64_t(row - min(q0, row)) + int64_t(ke - ks) - int64_t(max(q1, q0) - q0);
             lo = int(ks);
             hi = int(ke);
             if (g.mask != GAT_B200_MASK_FULL) {
@@ -180,6 +245,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             pos = int(max(int64_t(-INT32_MAX), min(at, int64_t(INT32_MAX))));
         }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_holder;
+    if (warp >= 4) {
         const bool some = hi > lo;
         const unsigned min_lo = __reduce_min_sync(0xffffffffu, some ? unsigned(lo) : 0xffffffffu);
         const unsigned max_hi = __reduce_max_sync(0xffffffffu, some ? unsigned(hi) : 0u);
@@ -193,33 +264,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     __syncthreads();
-    const unsigned first_key = min(range[0], range[4]), end_key = max(range[1], range[5]);
+    // key blocks [from, to) that tile t works on; blocks inside [max_lo, min_hi)
+    // are seen whole by every row that sees anything
+    unsigned first_key = range[0], end_key = range[1], max_lo = range[2], min_hi = range[3];
+    if constexpr (kTiles == 2) {
+        first_key = min(first_key, range[4]);
+        end_key = max(end_key, range[5]);
+        max_lo = max(max_lo, range[6]);
+        min_hi = min(min_hi, range[7]);
+    }
     const int blocks = end_key > first_key ? int((end_key - first_key + kRows - 1) / kRows) : 0;
-    // key blocks [from, to) that tile t works on
-    int from[2], to[2];
+    int from[kTiles], to[kTiles];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < kTiles; ++t) {
         const bool any = range[4 * t + 1] > range[4 * t];
         from[t] = any ? int((range[4 * t] - first_key) / kRows) : 0;
         to[t] = any ? int((range[4 * t + 1] - first_key + kRows - 1) / kRows) : 0;
     }
-    const int last_tile = to[1] > 0 ? 1 : 0;
-    // blocks [clean_from, clean_to) are seen whole by every row that sees anything
-    const unsigned max_lo = max(range[2], range[6]), min_hi = min(range[3], range[7]);
+    const int last_tile = to[kTiles - 1] > 0 ? kTiles - 1 : 0;
     const int ksteps = (g.dim + 15) / 16;
-    // 384 threads start with 168 registers (64,512): 128 x 72 + 256 x 216 of them afterwards
     if (warp < 4) {
+    // the roles leave registers to the softmax: 128 x 56 + 128 x 200 of 256 x 128 (one tile),
+    // 128 x 72 + 256 x 216 of 384 x 168 (two)
+    if constexpr (kTiles == 1)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    else
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (blocks == 0) {
-        // nothing to see: the softmax warps write zeros
-    } else if (warp == 0) {
+    if (warp == 0) {
         if (lane == 0) {
-            const int boxes = g.dim > 64 ? 2 : 1;
-            const uint32_t bytes = uint32_t(boxes) * kRows * 128;
-            mbar_expect_tx(q_full, bytes * (last_tile + 1));
-            for (int t = 0; t <= last_tile; ++t)
-                for (int b = 0; b < boxes; ++b)
-                    tma_load_3d(q_s + t * kTile + b * (kRows * 128), &tm_q, q_full, b * 64, head, int(row0) + t * kRows);
             bool ok = true;
             int j = 0;
             for (; j < blocks && ok; ++j) {
@@ -254,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = -1; j < blocks && ok; ++j) {
             const int s = j % kSt, sn = (j + 1) % kSt;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < kTiles; ++t) {
                 if (t > last_tile || !ok) break;
                 const bool now = j >= from[t] && j < to[t], next = j + 1 >= from[t] && j + 1 < to[t];
                 if (j >= 0) {
@@ -267,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (now) {
 #pragma unroll
                             for (int ks = 0; ks < kRows / 16; ++ks)
-                                mma_bf16_ts(tmem + 256 + 128 * t, tmem + 128 * t + ks * 8, vdesc + ks * 128, idesc_o);
+                                mma_bf16_ts(tmem + kO + DP * t, tmem + 128 * t + ks * 8, vdesc + ks * 128, idesc_o);
                             if (j + 1 == to[t]) mma_commit(o_full + t);
                         }
                         if (t == last_tile) mma_commit(v_empty + s);
@@ -297,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         // whatever was issued has finished before the CTA ends (v_empty of the last block)
-        if (ok)
+        if (ok && blocks > 0)
             mbar_wait_warp(v_empty + (blocks - 1) % kSt, uint32_t((blocks - 1) / kSt) & 1u, abort_flag, &g_attention_error);
     } else if (warp < 4) {
         // ---- V of masked blocks: non-finite values out, their keys noted ----
@@ -310,10 +382,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int half = warp - 2;  // 64 keys a warp
                 if (lane < 2) words[2 * half + lane] = 0;
                 __syncwarp();
-                const int boxes = g.dim > 64 ? 2 : 1;
                 for (int b = 0; b < boxes; ++b) {
                     uint8_t* base = v_s + s * kTile + b * (kRows * 128) + half * 64 * 128;
-#pragma unroll 4
+#pragma unroll 2
                     for (int i = lane; i < 64 * 8; i += 32) {
                         uint4 w = *reinterpret_cast<const uint4*>(base + i * 16);
                         auto hit = [](uint32_t x) {
@@ -339,12 +410,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    const int my_from = tile ? from[1] : from[0], my_to = tile ? to[1] : to[0];
+    if constexpr (kTiles == 1)
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    else
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int my_from = kTiles == 2 && tile ? from[kTiles - 1] : from[0], my_to = kTiles == 2 && tile ? to[kTiles - 1] : to[0];
     if (my_to > 0) {
         // ---- softmax of one tile: thread = row ----
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-        const uint32_t s_t = tmem + lanes + 128 * tile, o_t = tmem + lanes + 256 + 128 * tile;
+        const uint32_t s_t = tmem + lanes + 128 * tile, o_t = tmem + lanes + kO + DP * tile;
         const float nslope = BIAS ? -g.slopes[head] * kLog2e : 0.f;
         {
             uint32_t z[32];
@@ -367,24 +441,64 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld64(s_t, z);
             tmem_ld64(s_t + 64, z + 64);
             if constexpr (CAP) {
+                float top = fabsf(z[0]);
 #pragma unroll
-                for (int c = 0; c < kRows; ++c) z[c] = g.zcap * tanh_of_log2(z[c] * g.zscale);
+                for (int c = 1; c + 1 < kRows; c += 2) top = max3(top, fabsf(z[c]), fabsf(z[c + 1]));
+                top = fmaxf(top, fabsf(z[kRows - 1]));
+                if (__all_sync(0xffffffffu, top <= g.small)) {
+                    const f32x2 sc = pack2(g.tscale, g.tscale);
+                    f32x2 k[5];
+#pragma unroll
+                    for (int i = 0; i < 5; ++i) k[i] = pack2(g.tanh[i], g.tanh[i]);
+#pragma unroll
+                    for (int c = 0; c < kRows; c += 2) {
+                        const f32x2 t = mul2(pack2(z[c], z[c + 1]), sc), u = mul2(t, t);
+                        f32x2 p = fma2(k[4], u, k[3]);
+                        p = fma2(p, u, k[2]);
+                        p = fma2(p, u, k[1]);
+                        p = fma2(p, u, k[0]);
+                        unpack2(mul2(p, t), z[c], z[c + 1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kRows; ++c) z[c] = g.zcap * tanh_of_log2(z[c] * g.zscale);
+                }
             }
             if constexpr (BIAS) {
-                const float rel = float(pos + jl);
+                const float rel = float(pos + jl);  // distance of column c: |rel - c|
+                if (__all_sync(0xffffffffu, rel >= float(kRows - 1))) {
+                    const float base = nslope * rel;
 #pragma unroll
-                for (int c = 0; c < kRows; ++c) {
-                    if constexpr (!CAP) z[c] *= g.zscale;
-                    z[c] = fmaf(nslope, fabsf(rel - float(c)), z[c]);
+                    for (int c = 0; c < kRows; ++c) {
+                        const float e = fmaf(float(-c), nslope, base);
+                        z[c] = CAP ? z[c] + e : fmaf(z[c], g.zscale, e);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kRows; ++c) {
+                        const float e = nslope * fabsf(rel - float(c));
+                        z[c] = CAP ? z[c] + e : fmaf(z[c], g.zscale, e);
+                    }
                 }
             }
             if (!whole) {
+                // bit c of word w: column 32 w + c is visible
 #pragma unroll
-                for (int c = 0; c < kRows; ++c) z[c] = c >= jl && c < jh ? z[c] : -INFINITY;
+                for (int w = 0; w < 4; ++w) {
+                    const int b = min(max(jl - 32 * w, 0), 32), e = min(max(jh - 32 * w, 0), 32);
+                    const uint32_t bits = (e > b) ? ((e == 32 ? 0u : (1u << e)) - (1u << b)) : 0u;
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) z[32 * w + c] = bits & (1u << c) ? z[32 * w + c] : -INFINITY;
+                }
             }
-            float mb = z[0];
+            float mb = z[0], mb2 = z[1];
 #pragma unroll
-            for (int c = 1; c < kRows; ++c) mb = fmaxf(mb, z[c]);
+            for (int c = 2; c + 3 < kRows; c += 4) {
+                mb = max3(mb, z[c], z[c + 1]);
+                mb2 = max3(mb2, z[c + 2], z[c + 3]);
+            }
+            mb = max3(mb, z[kRows - 2], z[kRows - 1]);
+            mb = fmaxf(mb, mb2);
             if constexpr (!CAP && !BIAS) mb *= g.zscale;
             if (m == -INFINITY) m = mb;
             const bool grow = mb > m + 8.f;
@@ -392,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float f = grow ? ex2(m - mb) : 1.f;
                 if (grow) m = mb;
                 l *= f;
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < DP; c += 32) {
                     float o[32];
                     tmem_ld32(o_t + c, o);
@@ -403,23 +517,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tmem_wait_st();
             }
             const float ref = m == -INFINITY ? 0.f : m;
+            const f32x2 nref = pack2(-ref, -ref), zs = pack2(g.zscale, g.zscale);
             uint32_t p[kRows / 2];
-            float sum0 = 0.f, sum1 = 0.f;
+            f32x2 sum = pack2(0.f, 0.f), sum2 = sum;
 #pragma unroll
             for (int c = 0; c < kRows; c += 2) {
+                const f32x2 s2 = pack2(z[c], z[c + 1]);
                 float p0, p1;
-                if constexpr (CAP || BIAS) {
-                    p0 = ex2(z[c] - ref);
-                    p1 = ex2(z[c + 1] - ref);
-                } else {
-                    p0 = ex2(fmaf(z[c], g.zscale, -ref));
-                    p1 = ex2(fmaf(z[c + 1], g.zscale, -ref));
-                }
-                sum0 += p0;
-                sum1 += p1;
+                unpack2(CAP || BIAS ? add2(s2, nref) : fma2(s2, zs, nref), p0, p1);
+                p0 = ex2(p0);
+                p1 = ex2(p1);
+                if (c & 2)
+                    sum = add2(sum, pack2(p0, p1));
+                else
+                    sum2 = add2(sum2, pack2(p0, p1));
                 p[c / 2] = pack_bf16x2(p0, p1);
             }
-            l += sum0 + sum1;
+            {
+                float s0, s1;
+                unpack2(add2(sum, sum2), s0, s1);
+                l += s0 + s1;
+            }
             tmem_st32(s_t, p);
             tmem_st32(s_t + 32, p + 32);
             if (unsigned(key) < max_lo || unsigned(key) + kRows > min_hi) {
@@ -502,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     if (warp == 1) {
         fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Shape<DP>::kTmem));
     }
 }
 
@@ -515,13 +633,12 @@ int heads_map(CUtensorMap* m, const void* base, int dim, int heads, uint64_t row
 
 template <int DP, bool CAP, bool BIAS>
 int launch(const AttnArgs& g, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
-    constexpr int kSt = DP == 64 ? 4 : 2;
-    constexpr int smem = (2 + 2 * kSt) * kRows * DP * 2 + 1024 + 512;
+    constexpr int smem = Shape<DP>::kSmem, rows = Shape<DP>::kTiles * kRows;
     auto kern = attention_kernel<DP, CAP, BIAS>;
     GATB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    const uint64_t grid = (g.n_q + 2 * kRows - 1) / (2 * kRows) * uint64_t(g.heads);
+    const uint64_t grid = (g.n_q + rows - 1) / rows * uint64_t(g.heads);
     if (grid > uint64_t(INT32_MAX)) return fail("masked_attention: too many rows times heads");
-    kern<<<unsigned(grid), kThreads, smem, st>>>(q, k, v, g);
+    kern<<<unsigned(grid), Shape<DP>::kThreads, smem, st>>>(q, k, v, g);
     GATB_LAUNCH("masked_attention kernel");
     return 0;
 }
@@ -583,6 +700,9 @@ int masked_attention_launch(const AttentionShape& s, int nseg, uint64_t n_q, uin
     g.ldv = ldv;
     g.zscale = s.cap > 0.f ? 2.f * kLog2e * s.scale / s.cap : s.scale * kLog2e;
     g.zcap = s.cap * kLog2e;
+    g.tscale = s.cap > 0.f ? s.scale / s.cap : 0.f;
+    g.small = s.cap > 0.f ? kTanhLimit * s.cap / s.scale : 0.f;
+    for (int i = 0; i < 5; ++i) g.tanh[i] = kTanh[i] * g.zcap;
     g.out = static_cast<uint16_t*>(out);
     g.ldo = ldo;
     g.lse = lse;
