@@ -12,20 +12,27 @@
 // above, shared memory holds one CTA and it has two tiles. Either way one
 // tile's softmax runs beside the other's MMAs. Warps:
 //   0     TMA producer: Q once, K and V blocks through rings.
-//   1     MMA issuer: S = Q K^T into TMEM; O += P V with P read from TMEM (P
-//         overlays S).
+//   1     MMA issuer: S = Q K^T into TMEM; O += P V with P read from TMEM. With
+//         one tile P has columns of its own and the next S is computed while
+//         the softmax is at work; with two, P overlays S.
 //   2-3   masked blocks only: take non-finite values of V out of shared memory
 //         (a weight of zero times Inf or NaN is NaN) and note their keys; rows
 //         that do see such a key add it themselves.
-//   4 ..  softmax, four warps a tile, a row per thread: no shuffles.
-// The running maximum is only moved when it grows by more than 8 (a factor of
-// 256 in the weights, far inside FP32 and BF16's range), so O is seldom rescaled.
-// MMAs of a CTA run in order, so S's barrier also says that the tile's last P V
-// is done and O is at rest. P is rounded to BF16 (the tensor cores' input type;
+//   4 ..  softmax, a row per thread (no shuffles), four warps a tile; eight, two
+//         threads a row, where the weights need no common maximum (see below).
+// The running maximum is only moved when it grows by more than 24 (weights up
+// to 2^24, far inside FP32 and BF16's range), so O is seldom rescaled.
+// MMAs of a CTA run in order, so where P overlays S, S's barrier also says that
+// the tile's last P V is done and O is at rest. P is rounded to BF16 (the tensor cores' input type;
 // the sum keeps the unrounded FP32 weights).
 // The exponentials bound it (16 a clock and SM; a 128 x 128 block of dim 128
 // takes the tensor cores as long as its exponentials): the cap's tanh is a
-// polynomial on the FMA pipe wherever a block's scores stay below 0.6 cap.
+// polynomial on the FMA pipe wherever a block's scores stay below 0.6 cap. Capped
+// scores without a bias lie within +-cap, so up to a cap of 55 their weights
+// are taken relative to cap / 2 instead of the running maximum (2^-120 .. 2^40
+// and their sums are ordinary FP32 and BF16 numbers): no pass for the maximum,
+// no rescaling, 32 columns at a time flow from S to P and two threads share a
+// row. (With a maximum to agree on, two threads a row were slower than one.)
 #include <cuda.h>
 
 #include "attention.cuh"
@@ -87,6 +94,38 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
         : "memory");
 }
 
+// 32 lanes x 32 columns: the load, and the wait after which r may be read.
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, float* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+          "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+          "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32_wait(float* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+                   "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]),
+                   "+f"(r[15]), "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]),
+                   "+f"(r[22]), "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]),
+                   "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
 // Segments of the 32 consecutive rows first + lane (a converged warp): the
 // first row's by a 32-way search, the others' from the row pointers behind it.
 __device__ __forceinline__ int segment_of_lane(const uint64_t* row, int nseg, uint64_t first, int lane) {
@@ -118,6 +157,13 @@ __device__ __forceinline__ f32x2 pack2(float x, float y) {
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
     return r;
 }
+// A constant pair that stays in registers (the compiler would otherwise put it
+// together again at each use).
+__device__ __forceinline__ f32x2 pair_of(float x) {
+    f32x2 r;
+    asm volatile("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(x));
+    return r;
+}
 __device__ __forceinline__ void unpack2(f32x2 v, float& x, float& y) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
 }
@@ -142,34 +188,57 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
+// Bits of the columns [b, e) of 32.
+__device__ __forceinline__ uint32_t visible(int b, int e) {
+    b = min(max(b, 0), 32);
+    e = min(max(e, 0), 32);
+    return e > b ? (e == 32 ? 0u : (1u << e)) - (1u << b) : 0u;
+}
+
+// Growth of the maximum (log2) up to which the reference stays.
+constexpr float kGrow = 24.f;
+// Largest cap * log2 e whose weights are taken relative to half of it.
+constexpr float kFixedCap = 80.f;
 // tanh(x) = x p(x^2) for |x| <= 0.6, relative error 7.4e-8 (minimax, Remez exchange).
 constexpr float kTanhLimit = 0.6f;
 constexpr float kTanh[5] = {0.999999926872f, -0.333323099889f, 0.133101737673f, -0.0521014822761f, 0.0154754278422f};
 
 // DP: dim rounded up to 64 or 128. CAP / BIAS: scores go through the tanh / get the distance bias.
-// TMEM: S / P of tile t at 128 t, O of tile t at 128 TILES + DP t.
-template <int DP>
+// FIXED: weights relative to half the cap (capped scores without a bias).
+// TMEM, one tile: S at 0, P at 128, O at 192; two: S and P of tile t at 128 t, O at 256 + 128 t.
+template <int DP, bool FIXED>
 struct Shape {
     static constexpr int kTiles = DP == 64 ? 1 : 2;
-    static constexpr int kThreads = 128 + 128 * kTiles;
+    static constexpr int kHalves = FIXED ? 2 : 1;        // softmax threads a row
+    static constexpr int kThreads = 128 + 128 * kTiles * kHalves;
     static constexpr int kCtas = DP == 64 ? 2 : 1;       // per SM
+    // registers after setmaxnreg, inside the launch's kCtas * kThreads * (65536 / (kCtas * kThreads), whole eights)
+    static constexpr int kRoleRegs = kTiles * kHalves == 1 || FIXED ? 56 : 72;
+    static constexpr int kSoftmaxRegs = FIXED ? (DP == 64 ? 88 : 104) : (DP == 64 ? 200 : 216);
+    static constexpr int kLaunchRegs = 65536 / (kCtas * kThreads) / 8 * 8;
+    static_assert(128 * kRoleRegs + 128 * kTiles * kHalves * kSoftmaxRegs <= kThreads * kLaunchRegs, "register split");
     static constexpr int kTmem = DP == 64 ? 256 : 512;
     static constexpr int kTile = kRows * DP * 2;         // bytes of a Q tile, a K block, a V block
     static constexpr int kStages = 2;                    // K and V stages
-    static constexpr int kSmem = (kTiles + 2 * kStages) * kTile + 1024 + 512;
+    static constexpr int kSmem = (kTiles + 2 * kStages) * kTile + (FIXED ? kTiles * 2 * kRows * 4 : 0) + 1024 + 512;
 };
-template <int DP, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
+template <int DP, bool CAP, bool BIAS, bool FIXED>
+__global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::kCtas)
     attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnArgs g) {
-    constexpr int kTiles = Shape<DP>::kTiles, kTile = Shape<DP>::kTile, kSt = Shape<DP>::kStages;
-    constexpr uint32_t kO = 128 * kTiles;
+    constexpr int kTiles = Shape<DP, FIXED>::kTiles, kHalves = Shape<DP, FIXED>::kHalves, kTile = Shape<DP, FIXED>::kTile, kSt = Shape<DP, FIXED>::kStages;
+    static_assert(!FIXED || (CAP && !BIAS), "only capped scores are bounded");
+    constexpr bool kOwnP = kTiles == 1;
+    // P's columns for the block's keys 64 and up start kPHalf behind the others: where P overlays S, each
+    // half of P lies in its own half of S
+    constexpr uint32_t kP = kOwnP ? 128 : 0, kPHalf = kOwnP ? 32 : 64, kO = kOwnP ? 192 : 256;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* q_s = smem;
     uint8_t* k_s = q_s + kTiles * kTile;
     uint8_t* v_s = k_s + kSt * kTile;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + kSt * kTile);
+    float* sums = reinterpret_cast<float*>(v_s + kSt * kTile);  // FIXED: [kTiles][2][kRows]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sums + (FIXED ? kTiles * 2 * kRows : 0));
     uint64_t* q_full = bars;
     uint64_t* k_full = bars + 1;
     uint64_t* k_empty = k_full + kSt;
@@ -179,7 +248,10 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
     uint64_t* s_full = v_empty + kSt;    // [kTiles]
     uint64_t* p_full = s_full + kTiles;  // [kTiles]
     uint64_t* o_full = p_full + kTiles;  // [kTiles]
-    uint32_t* bad = reinterpret_cast<uint32_t*>(o_full + kTiles);  // [kSt][4] keys of the block with non-finite values
+    uint64_t* s_read = o_full + kTiles;  // own P: S is in registers
+    uint64_t* pv_done = s_read + 1;      // own P: P and O are at rest
+    uint64_t* pairs = pv_done + 1;       // FIXED: [kTiles][4], the two warps of the same rows
+    uint32_t* bad = reinterpret_cast<uint32_t*>(pairs + 4 * kTiles);  // [kSt][4] keys of the block with non-finite values
     unsigned* range = bad + 4 * kSt;  // per tile: smallest lo, largest hi, largest lo, smallest hi
     uint32_t* tmem_holder = range + 4 * kTiles;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
@@ -202,13 +274,16 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
         }
         for (int t = 0; t < kTiles; ++t) {
             mbar_init(s_full + t, 1);
-            mbar_init(p_full + t, 4);
+            mbar_init(p_full + t, 4 * kHalves);
+            for (int i = 0; i < 4; ++i) mbar_init(pairs + 4 * t + i, 2);
             mbar_init(o_full + t, 1);
             range[4 * t] = 0xffffffffu;
             range[4 * t + 1] = 0;
             range[4 * t + 2] = 0;
             range[4 * t + 3] = 0xffffffffu;
         }
+        mbar_init(s_read, 4 * kHalves);
+        mbar_init(pv_done, 1);
         *abort_flag = 0;
         fence_mbarrier_init();
         mbar_expect_tx(q_full, bytes * q_tiles);
@@ -219,12 +294,13 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
     if (warp == 1) {
         __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
-                     "r"(Shape<DP>::kTmem));
+                     "r"(Shape<DP, FIXED>::kTmem));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
 
     // The row's key interval (softmax threads), its position and the tile's ranges.
-    const int tile = warp >= 8 ? 1 : 0;
+    const int half = kHalves == 2 ? ((warp - 4) >> 2) & 1 : 0;
+    const int tile = kTiles == 2 && warp >= 4 + 4 * kHalves ? 1 : 0;
     const int r = (warp & 3) * 32 + lane;
     const uint64_t row = row0 + uint64_t(tile) * kRows + r;
     int lo = 0, hi = 0, pos = 0;
@@ -284,12 +360,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
     const int last_tile = to[kTiles - 1] > 0 ? kTiles - 1 : 0;
     const int ksteps = (g.dim + 15) / 16;
     if (warp < 4) {
-    // the roles leave registers to the softmax: 128 x 56 + 128 x 200 of 256 x 128 (one tile),
-    // 128 x 72 + 256 x 216 of 384 x 168 (two)
-    if constexpr (kTiles == 1)
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    else
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Shape<DP, FIXED>::kRoleRegs));
     if (warp == 0) {
         if (lane == 0) {
             bool ok = true;
@@ -322,49 +393,84 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
         const uint32_t idesc_s = idesc_bf16(kRows, kRows, 0, 0);
         const uint32_t idesc_o = idesc_bf16(kRows, ksteps * 16, 0, 1);
         bool ok = mbar_wait_warp(q_full, 0, abort_flag, &g_attention_error);
-        uint32_t used[2] = {0, 0};  // blocks of tile t issued so far
-        for (int j = -1; j < blocks && ok; ++j) {
-            const int s = j % kSt, sn = (j + 1) % kSt;
+        auto scores = [&](int t, int s) {
+            const uint64_t qdesc = desc_sw128(smem_u32(q_s + t * kTile), 16, 1024);
+            const uint64_t kdesc = desc_sw128(smem_u32(k_s + s * kTile), 16, 1024);
 #pragma unroll
-            for (int t = 0; t < kTiles; ++t) {
-                if (t > last_tile || !ok) break;
-                const bool now = j >= from[t] && j < to[t], next = j + 1 >= from[t] && j + 1 < to[t];
-                if (j >= 0) {
-                    if (t == 0) ok = mbar_wait_warp(v_ready + s, uint32_t(j / kSt) & 1u, abort_flag, &g_attention_error);
-                    if (ok && now) ok = mbar_wait_warp(p_full + t, used[t]++ & 1u, abort_flag, &g_attention_error);
+            for (int ks = 0; ks < DP / 16; ++ks) {
+                if (ks >= ksteps) break;
+                const uint32_t off = (ks >> 2) * (kRows * 128 / 16) + (ks & 3) * 2;
+                mma_bf16(tmem + 128 * t, qdesc + off, kdesc + off, idesc_s, ks > 0);
+            }
+            mma_commit(s_full + t);
+        };
+        auto values = [&](int t, int s) {
+            const uint64_t vdesc = desc_sw128(smem_u32(v_s + s * kTile), kRows * 128, 1024);
+#pragma unroll
+            for (int ks = 0; ks < kRows / 16; ++ks)
+                mma_bf16_ts(tmem + kO + DP * t, tmem + kP + 128 * t + (ks >> 2) * kPHalf + (ks & 3) * 8, vdesc + ks * 128, idesc_o);
+        };
+        if constexpr (kOwnP) {
+            for (int j = -1; j < blocks && ok; ++j) {
+                if (j + 1 < blocks) {
+                    const int s = (j + 1) % kSt;
+                    ok = mbar_wait_warp(k_full + s, uint32_t((j + 1) / kSt) & 1u, abort_flag, &g_attention_error) &&
+                         (j < 0 || mbar_wait_warp(s_read, uint32_t(j) & 1u, abort_flag, &g_attention_error));
                     if (!ok) break;
                     fence_after();
-                    const uint64_t vdesc = desc_sw128(smem_u32(v_s + s * kTile), kRows * 128, 1024);
                     if (elect_one()) {
-                        if (now) {
-#pragma unroll
-                            for (int ks = 0; ks < kRows / 16; ++ks)
-                                mma_bf16_ts(tmem + kO + DP * t, tmem + 128 * t + ks * 8, vdesc + ks * 128, idesc_o);
-                            if (j + 1 == to[t]) mma_commit(o_full + t);
-                        }
-                        if (t == last_tile) mma_commit(v_empty + s);
+                        scores(0, s);
+                        mma_commit(k_empty + s);
                     }
                     __syncwarp();
                 }
-                if (j + 1 < blocks) {
-                    if (t == 0) ok = mbar_wait_warp(k_full + sn, uint32_t((j + 1) / kSt) & 1u, abort_flag, &g_attention_error);
+                if (j >= 0) {
+                    const int s = j % kSt;
+                    ok = mbar_wait_warp(v_ready + s, uint32_t(j / kSt) & 1u, abort_flag, &g_attention_error) &&
+                         mbar_wait_warp(p_full, uint32_t(j) & 1u, abort_flag, &g_attention_error);
                     if (!ok) break;
                     fence_after();
-                    const uint64_t qdesc = desc_sw128(smem_u32(q_s + t * kTile), 16, 1024);
-                    const uint64_t kdesc = desc_sw128(smem_u32(k_s + sn * kTile), 16, 1024);
                     if (elect_one()) {
-                        if (next) {
-#pragma unroll
-                            for (int ks = 0; ks < DP / 16; ++ks) {
-                                if (ks >= ksteps) break;
-                                const uint32_t off = (ks >> 2) * (kRows * 128 / 16) + (ks & 3) * 2;
-                                mma_bf16(tmem + 128 * t, qdesc + off, kdesc + off, idesc_s, ks > 0);
-                            }
-                            mma_commit(s_full + t);
-                        }
-                        if (t == last_tile) mma_commit(k_empty + sn);
+                        values(0, s);
+                        mma_commit(pv_done);
+                        mma_commit(v_empty + s);
+                        if (j + 1 == blocks) mma_commit(o_full);
                     }
                     __syncwarp();
+                }
+            }
+        } else {
+            uint32_t used[2] = {0, 0};  // blocks of tile t issued so far
+            for (int j = -1; j < blocks && ok; ++j) {
+                const int s = j % kSt, sn = (j + 1) % kSt;
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) {
+                    if (t > last_tile || !ok) break;
+                    const bool now = j >= from[t] && j < to[t], next = j + 1 >= from[t] && j + 1 < to[t];
+                    if (j >= 0) {
+                        if (t == 0) ok = mbar_wait_warp(v_ready + s, uint32_t(j / kSt) & 1u, abort_flag, &g_attention_error);
+                        if (ok && now) ok = mbar_wait_warp(p_full + t, used[t]++ & 1u, abort_flag, &g_attention_error);
+                        if (!ok) break;
+                        fence_after();
+                        if (elect_one()) {
+                            if (now) {
+                                values(t, s);
+                                if (j + 1 == to[t]) mma_commit(o_full + t);
+                            }
+                            if (t == last_tile) mma_commit(v_empty + s);
+                        }
+                        __syncwarp();
+                    }
+                    if (j + 1 < blocks) {
+                        if (t == 0) ok = mbar_wait_warp(k_full + sn, uint32_t((j + 1) / kSt) & 1u, abort_flag, &g_attention_error);
+                        if (!ok) break;
+                        fence_after();
+                        if (elect_one()) {
+                            if (next) scores(t, sn);
+                            if (t == last_tile) mma_commit(k_empty + sn);
+                        }
+                        __syncwarp();
+                    }
                 }
             }
         }
@@ -375,7 +481,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
         // ---- V of masked blocks: non-finite values out, their keys noted ----
         for (int j = 0; j < blocks; ++j) {
             const int s = j % kSt;
-            if (!mbar_wait(v_full + s, uint32_t(j / kSt) & 1u, abort_flag, &g_attention_error)) break;
+            if (!mbar_wait_warp(v_full + s, uint32_t(j / kSt) & 1u, abort_flag, &g_attention_error)) break;
             const unsigned key = first_key + unsigned(j) * kRows;
             if (key < max_lo || key + kRows > min_hi) {
                 uint32_t* words = bad + 4 * s;
@@ -410,53 +516,141 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
         }
     }
     } else {
-    if constexpr (kTiles == 1)
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    else
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape<DP, FIXED>::kSoftmaxRegs));
     const int my_from = kTiles == 2 && tile ? from[kTiles - 1] : from[0], my_to = kTiles == 2 && tile ? to[kTiles - 1] : to[0];
     if (my_to > 0) {
-        // ---- softmax of one tile: thread = row ----
+        // ---- softmax of one tile: thread = row (FIXED: half the columns of a row, of S, P and O) ----
+        constexpr int kOCols = DP / kHalves;
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-        const uint32_t s_t = tmem + lanes + 128 * tile, o_t = tmem + lanes + kO + DP * tile;
+        const uint32_t s_t = tmem + lanes + 128 * tile, p_t = s_t + kP, o_t = tmem + lanes + kO + DP * tile + kOCols * half;
         const float nslope = BIAS ? -g.slopes[head] * kLog2e : 0.f;
         {
             uint32_t z[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) z[i] = 0;
 #pragma unroll
-            for (int c = 0; c < DP; c += 32) tmem_st32(o_t + c, z);
+            for (int c = 0; c < kOCols; c += 32) tmem_st32(o_t + c, z);
             tmem_wait_st();
         }
-        float m = -INFINITY, l = 0.f;  // reference maximum (log2 units) and sum of weights
+        f32x2 sc = 0, tk[5] = {};  // the tanh's scale and polynomial
+        if constexpr (CAP) {
+            sc = pair_of(g.tscale);
+#pragma unroll
+            for (int i = 0; i < 5; ++i) tk[i] = pair_of(g.tanh[i]);
+        }
+        // the reference maximum (log2 units) and the sum of the weights
+        float m = FIXED ? 0.5f * g.zcap : -INFINITY, l = 0.f;
+        // the intervals of the warp's rows that see anything: smallest and largest begin and end
+        const bool some = hi > lo;
+        const int lo_min = __reduce_min_sync(0xffffffffu, some ? lo : INT32_MAX);
+        const int lo_max = __reduce_max_sync(0xffffffffu, some ? lo : 0);
+        const int hi_min = __reduce_min_sync(0xffffffffu, some ? hi : INT32_MAX);
+        const int hi_max = __reduce_max_sync(0xffffffffu, some ? hi : 0);
+        uint32_t met = 0;
+        auto meet_pair = [&] {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pairs + 4 * tile + (warp & 3));
+            return mbar_wait_warp(pairs + 4 * tile + (warp & 3), met++ & 1u, abort_flag, &g_attention_error);
+        };
         bool ok = true;
         uint32_t use = 0;
         for (int j = my_from; j < my_to; ++j, ++use) {
-            if (!mbar_wait(s_full + tile, use & 1u, abort_flag, &g_attention_error)) { ok = false; break; }
+            if (!mbar_wait_warp(s_full + tile, use & 1u, abort_flag, &g_attention_error)) { ok = false; break; }
             fence_after();
             const int key = int(first_key) + j * kRows;
             const int jl = lo - key, jh = hi - key;  // visible columns [jl, jh)
-            const bool whole = __all_sync(0xffffffffu, (jl <= 0 && jh >= kRows) || hi <= lo);
+            // 32-column words of the block: 0 nobody sees, 1 seen in part, 2 seen whole
+            auto seen = [&](int w) {
+                const int a = key + 32 * w, b = a + 32;
+                return b <= lo_min || a >= hi_max ? 0 : a >= lo_max && b <= hi_min ? 2 : 1;
+            };
+            // S may be overwritten once it is in registers; P and O may be touched once the last P V is done
+            auto s_is_read = [&] {
+                if constexpr (kOwnP) {
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_read);
+                }
+            };
+            auto p_is_free = [&] {
+                return !kOwnP || use == 0 || mbar_wait_warp(pv_done, (use - 1) & 1u, abort_flag, &g_attention_error);
+            };
+            if constexpr (FIXED) {
+                f32x2 sum = pack2(0.f, 0.f), sum2 = sum;
+                const f32x2 nref = pack2(-m, -m);
+                if (!p_is_free()) { ok = false; break; }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int w = 2 * half + i;
+                    float x[32];
+                    tmem_ld32(s_t + 32 * w, x);
+                    if (i == 1) s_is_read();
+                    uint32_t p[16];
+                    const int sw = seen(w);
+                    if (sw == 0) {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) p[c] = 0;
+                        tmem_st16(p_t + kPHalf * half + 16 * i, p);
+                        continue;
+                    }
+                    float top = fabsf(x[0]);
+#pragma unroll
+                    for (int c = 1; c < 31; c += 2) top = max3(top, fabsf(x[c]), fabsf(x[c + 1]));
+                    top = fmaxf(top, fabsf(x[31]));
+                    if (__all_sync(0xffffffffu, top <= g.small)) {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            const f32x2 t = mul2(pack2(x[c], x[c + 1]), sc), u = mul2(t, t);
+                            f32x2 k = fma2(tk[4], u, tk[3]);
+                            k = fma2(k, u, tk[2]);
+                            k = fma2(k, u, tk[1]);
+                            k = fma2(k, u, tk[0]);
+                            unpack2(fma2(k, t, nref), x[c], x[c + 1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) x[c] = fmaf(g.zcap, tanh_of_log2(x[c] * g.zscale), -m);
+                    }
+                    if (sw == 1) {
+                        const uint32_t bits = visible(jl - 32 * w, jh - 32 * w);
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) x[c] = bits & (1u << c) ? x[c] : -INFINITY;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2) {
+                        const float p0 = ex2(x[c]), p1 = ex2(x[c + 1]);
+                        if (c & 2)
+                            sum = add2(sum, pack2(p0, p1));
+                        else
+                            sum2 = add2(sum2, pack2(p0, p1));
+                        p[c / 2] = pack_bf16x2(p0, p1);
+                    }
+                    tmem_st16(p_t + kPHalf * half + 16 * i, p);
+                }
+                float s0, s1;
+                unpack2(add2(sum, sum2), s0, s1);
+                l += s0 + s1;
+            } else {
             float z[kRows];
-            tmem_ld64(s_t, z);
-            tmem_ld64(s_t + 64, z + 64);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) tmem_ld32_start(s_t + 32 * w, z + 32 * w);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) tmem_ld32_wait(z + 32 * w);
+            s_is_read();
+            const bool whole = key >= lo_max && key + kRows <= hi_min;
             if constexpr (CAP) {
                 float top = fabsf(z[0]);
 #pragma unroll
                 for (int c = 1; c + 1 < kRows; c += 2) top = max3(top, fabsf(z[c]), fabsf(z[c + 1]));
                 top = fmaxf(top, fabsf(z[kRows - 1]));
                 if (__all_sync(0xffffffffu, top <= g.small)) {
-                    const f32x2 sc = pack2(g.tscale, g.tscale);
-                    f32x2 k[5];
-#pragma unroll
-                    for (int i = 0; i < 5; ++i) k[i] = pack2(g.tanh[i], g.tanh[i]);
 #pragma unroll
                     for (int c = 0; c < kRows; c += 2) {
                         const f32x2 t = mul2(pack2(z[c], z[c + 1]), sc), u = mul2(t, t);
-                        f32x2 p = fma2(k[4], u, k[3]);
-                        p = fma2(p, u, k[2]);
-                        p = fma2(p, u, k[1]);
-                        p = fma2(p, u, k[0]);
+                        f32x2 p = fma2(tk[4], u, tk[3]);
+                        p = fma2(p, u, tk[2]);
+                        p = fma2(p, u, tk[1]);
+                        p = fma2(p, u, tk[0]);
                         unpack2(mul2(p, t), z[c], z[c + 1]);
                     }
                 } else {
@@ -482,11 +676,9 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
                 }
             }
             if (!whole) {
-                // bit c of word w: column 32 w + c is visible
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    const int b = min(max(jl - 32 * w, 0), 32), e = min(max(jh - 32 * w, 0), 32);
-                    const uint32_t bits = (e > b) ? ((e == 32 ? 0u : (1u << e)) - (1u << b)) : 0u;
+                    const uint32_t bits = visible(jl - 32 * w, jh - 32 * w);  // bit c: column 32 w + c is visible
 #pragma unroll
                     for (int c = 0; c < 32; ++c) z[32 * w + c] = bits & (1u << c) ? z[32 * w + c] : -INFINITY;
                 }
@@ -500,8 +692,9 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
             mb = max3(mb, z[kRows - 2], z[kRows - 1]);
             mb = fmaxf(mb, mb2);
             if constexpr (!CAP && !BIAS) mb *= g.zscale;
+            if (!p_is_free()) { ok = false; break; }
             if (m == -INFINITY) m = mb;
-            const bool grow = mb > m + 8.f;
+            const bool grow = mb > m + kGrow;
             if (__any_sync(0xffffffffu, grow)) {
                 const float f = grow ? ex2(m - mb) : 1.f;
                 if (grow) m = mb;
@@ -538,15 +731,20 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
                 unpack2(add2(sum, sum2), s0, s1);
                 l += s0 + s1;
             }
-            tmem_st32(s_t, p);
-            tmem_st32(s_t + 32, p + 32);
+            tmem_st32(p_t, p);
+            tmem_st32(p_t + kPHalf, p + 32);
+            }
             if (unsigned(key) < max_lo || unsigned(key) + kRows > min_hi) {
                 // keys with non-finite values that this row sees: their weights times those values
                 const int s = j % kSt;
-                if (!mbar_wait(v_ready + s, uint32_t(j / kSt) & 1u, abort_flag, &g_attention_error)) { ok = false; break; }
-                tmem_wait_st();
+                if (!mbar_wait_warp(v_ready + s, uint32_t(j / kSt) & 1u, abort_flag, &g_attention_error)) { ok = false; break; }
+                const bool any_bad = bad[4 * s] | bad[4 * s + 1] | bad[4 * s + 2] | bad[4 * s + 3];
+                if (any_bad) {  // the same for both warps of a row
+                    tmem_wait_st();
+                    if (kHalves == 2 && !meet_pair()) { ok = false; break; }  // both halves' weights are in P
+                }
 #pragma unroll 1
-                for (int w = 0; w < 4; ++w) {
+                for (int w = any_bad ? 0 : 4; w < 4; ++w) {
                     uint32_t bits = bad[4 * s + w];
                     while (bits) {  // the same for the whole warp
                         const int c = w * 32 + __ffs(bits) - 1;
@@ -555,19 +753,19 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
                         asm volatile(
                             "tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;"
                             : "=r"(pw)
-                            : "r"(s_t + c / 2)
+                            : "r"(p_t + (c >> 6) * kPHalf + (c & 63) / 2)
                             : "memory");
                         const float pc = (c & 1) ? bf16hi(pw) : bf16lo(pw);
                         const bool mine = c >= jl && c < jh;
                         const uint16_t* vr = g.v + (uint64_t(key) + c) * uint64_t(g.ldv) + uint64_t(kv_head) * g.dim;
 #pragma unroll 1
-                        for (int x = 0; x < DP; x += 8) {
+                        for (int x = 0; x < kOCols; x += 8) {
                             float o[8];
                             tmem_ld8(o_t + x, o);
 #pragma unroll
                             for (int i = 0; i < 8; ++i)
-                                if (mine && x + i < g.dim) {
-                                    const uint32_t e = vr[x + i];
+                                if (mine && kOCols * half + x + i < g.dim) {
+                                    const uint32_t e = vr[kOCols * half + x + i];
                                     if ((e & 0x7f80u) == 0x7f80u) o[i] += pc * bf16lo(e);
                                 }
                             const uint32_t* ou = reinterpret_cast<const uint32_t*>(o);
@@ -585,19 +783,25 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full + tile);
         }
-        if (ok && mbar_wait(o_full + tile, 0, abort_flag, &g_attention_error)) {
+        if (ok && mbar_wait_warp(o_full + tile, 0, abort_flag, &g_attention_error)) {
             fence_after();
+            if constexpr (kHalves == 2) {
+                float* s2 = sums + tile * 2 * kRows;
+                s2[half * kRows + r] = l;
+                meet_pair();
+                l = s2[r] + s2[kRows + r];
+            }
             const float inv = hi > lo ? 1.f / l : 0.f;
             const bool live = row < g.n_q;
-            uint16_t* orow = g.out + row * uint64_t(g.ldo) + uint64_t(head) * g.dim;
+            uint16_t* orow = g.out + row * uint64_t(g.ldo) + uint64_t(head) * g.dim + kOCols * half;
 #pragma unroll 1
-            for (int c = 0; c < DP; c += 32) {
+            for (int c = 0; c < kOCols; c += 32) {
                 float o[32];
                 tmem_ld32(o_t + c, o);
                 if (live) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
-                        if (c + i >= g.dim) break;
+                        if (kOCols * half + c + i >= g.dim) break;
                         uint32_t w[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
@@ -607,10 +811,10 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
                 }
                 __syncwarp();
             }
-            if (live && g.lse) g.lse[row * g.heads + head] = hi > lo ? (m + log2f(l)) * kLn2 : -INFINITY;
+            if (live && g.lse && half == 0) g.lse[row * g.heads + head] = hi > lo ? (m + log2f(l)) * kLn2 : -INFINITY;
         }
     }
-    if (my_to == 0 && row < g.n_q) {  // every row of the tile sees nothing
+    if (my_to == 0 && row < g.n_q && half == 0) {  // every row of the tile sees nothing
         uint16_t* orow = g.out + row * uint64_t(g.ldo) + uint64_t(head) * g.dim;
         for (int c = 0; c < g.dim; c += 8) *reinterpret_cast<uint4*>(orow + c) = make_uint4(0, 0, 0, 0);
         if (g.lse) g.lse[row * g.heads + head] = -INFINITY;
@@ -620,7 +824,7 @@ __global__ void __launch_bounds__(Shape<DP>::kThreads, Shape<DP>::kCtas)
     __syncthreads();
     if (warp == 1) {
         fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Shape<DP>::kTmem));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Shape<DP, FIXED>::kTmem));
     }
 }
 
@@ -631,22 +835,23 @@ int heads_map(CUtensorMap* m, const void* base, int dim, int heads, uint64_t row
     return make_tiled_map(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box, true);
 }
 
-template <int DP, bool CAP, bool BIAS>
+template <int DP, bool CAP, bool BIAS, bool FIXED>
 int launch(const AttnArgs& g, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
-    constexpr int smem = Shape<DP>::kSmem, rows = Shape<DP>::kTiles * kRows;
-    auto kern = attention_kernel<DP, CAP, BIAS>;
+    constexpr int smem = Shape<DP, FIXED>::kSmem, rows = Shape<DP, FIXED>::kTiles * kRows;
+    auto kern = attention_kernel<DP, CAP, BIAS, FIXED>;
     GATB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     const uint64_t grid = (g.n_q + rows - 1) / rows * uint64_t(g.heads);
     if (grid > uint64_t(INT32_MAX)) return fail("masked_attention: too many rows times heads");
-    kern<<<unsigned(grid), Shape<DP>::kThreads, smem, st>>>(q, k, v, g);
+    kern<<<unsigned(grid), Shape<DP, FIXED>::kThreads, smem, st>>>(q, k, v, g);
     GATB_LAUNCH("masked_attention kernel");
     return 0;
 }
 template <int DP>
 int launch(const AttnArgs& g, bool cap, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
            cudaStream_t st) {
-    if (cap) return g.slopes ? launch<DP, true, true>(g, q, k, v, st) : launch<DP, true, false>(g, q, k, v, st);
-    return g.slopes ? launch<DP, false, true>(g, q, k, v, st) : launch<DP, false, false>(g, q, k, v, st);
+    if (cap && !g.slopes && g.zcap <= kFixedCap) return launch<DP, true, false, true>(g, q, k, v, st);
+    if (cap) return g.slopes ? launch<DP, true, true, false>(g, q, k, v, st) : launch<DP, true, false, false>(g, q, k, v, st);
+    return g.slopes ? launch<DP, false, true, false>(g, q, k, v, st) : launch<DP, false, false, false>(g, q, k, v, st);
 }
 
 }  // namespace
