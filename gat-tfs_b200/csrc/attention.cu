@@ -62,9 +62,9 @@ struct AttnArgs {
     int ldv;
     float zscale;    // without a cap: scale * log2 e; with one: 2 log2 e * scale / cap
     float zcap;      // cap * log2 e
-    float tscale;    // scale / cap
-    float small;     // raw scores up to which the tanh's polynomial holds
-    float tanh[5];   // its coefficients times zcap
+    float small;     // raw scores up to which the tanh's long polynomial holds (half of it: the short one)
+    float tanh[5];   // coefficients of s, s^3 .. in zcap tanh(scale / cap * s)
+    float tanh3[3];
     uint16_t* out;
     int ldo;
     float* lse;
@@ -199,9 +199,15 @@ __device__ __forceinline__ uint32_t visible(int b, int e) {
 constexpr float kGrow = 24.f;
 // Largest cap * log2 e whose weights are taken relative to half of it.
 constexpr float kFixedCap = 80.f;
-// tanh(x) = x p(x^2) for |x| <= 0.6, relative error 7.4e-8 (minimax, Remez exchange).
+// tanh(x) = x p(x^2), minimax polynomials (Remez exchange): five terms for
+// |x| <= 0.6, relative error 7.4e-8, and three for |x| <= 0.3, 1.2e-6 (of a
+// score of at most 0.3 cap: 2.5e-5 in a weight's exponent at the very end).
 constexpr float kTanhLimit = 0.6f;
 constexpr float kTanh[5] = {0.999999926872f, -0.333323099889f, 0.133101737673f, -0.0521014822761f, 0.0154754278422f};
+constexpr float kTanhShort[3] = {0.99999883885f, -0.33310021606f, 0.126339459906f};
+// The coefficients take scale / cap into themselves, in powers up to the ninth:
+// outside this range of it the tanh is computed from exponentials.
+constexpr float kTanhScale = 8192.f;
 
 // DP: dim rounded up to 64 or 128. CAP / BIAS: scores go through the tanh / get the distance bias.
 // FIXED: weights relative to half the cap (capped scores without a bias).
@@ -532,11 +538,12 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
             for (int c = 0; c < kOCols; c += 32) tmem_st32(o_t + c, z);
             tmem_wait_st();
         }
-        f32x2 sc = 0, tk[5] = {};  // the tanh's scale and polynomial
+        f32x2 tk[5] = {}, tk3[3] = {};  // the tanh's polynomials
         if constexpr (CAP) {
-            sc = pair_of(g.tscale);
 #pragma unroll
-            for (int i = 0; i < 5; ++i) tk[i] = pair_of(g.tanh[i]);
+            for (int i = 0; i < 5; ++i) tk[i] = pack2(g.tanh[i], g.tanh[i]);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) tk3[i] = pair_of(g.tanh3[i]);
         }
         // the reference maximum (log2 units) and the sum of the weights
         float m = FIXED ? 0.5f * g.zcap : -INFINITY, l = 0.f;
@@ -579,12 +586,26 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                 f32x2 sum = pack2(0.f, 0.f), sum2 = sum;
                 const f32x2 nref = pack2(-m, -m);
                 if (!p_is_free()) { ok = false; break; }
+                float x2[2][32];
+                tmem_ld32_start(s_t + 64 * half, x2[0]);
+                tmem_ld32_start(s_t + 64 * half + 32, x2[1]);
+                tmem_ld32_wait(x2[0]);
+                tmem_ld32_wait(x2[1]);
+                s_is_read();
+                float top = 0.f, top2 = 0.f;
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    top = max3(top, fabsf(x2[0][c]), fabsf(x2[0][c + 1]));
+                    top2 = max3(top2, fabsf(x2[1][c]), fabsf(x2[1][c + 1]));
+                }
+                top = fmaxf(top, top2);
+                const int degree = __all_sync(0xffffffffu, top <= 0.5f * g.small) ? 3
+                                   : __all_sync(0xffffffffu, top <= g.small)      ? 5
+                                                                                  : 0;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int w = 2 * half + i;
-                    float x[32];
-                    tmem_ld32(s_t + 32 * w, x);
-                    if (i == 1) s_is_read();
+                    float* x = x2[i];
                     uint32_t p[16];
                     const int sw = seen(w);
                     if (sw == 0) {
@@ -593,14 +614,17 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                         tmem_st16(p_t + kPHalf * half + 16 * i, p);
                         continue;
                     }
-                    float top = fabsf(x[0]);
-#pragma unroll
-                    for (int c = 1; c < 31; c += 2) top = max3(top, fabsf(x[c]), fabsf(x[c + 1]));
-                    top = fmaxf(top, fabsf(x[31]));
-                    if (__all_sync(0xffffffffu, top <= g.small)) {
+                    if (degree == 3) {
 #pragma unroll
                         for (int c = 0; c < 32; c += 2) {
-                            const f32x2 t = mul2(pack2(x[c], x[c + 1]), sc), u = mul2(t, t);
+                            const f32x2 t = pack2(x[c], x[c + 1]), u = mul2(t, t);
+                            const f32x2 k = fma2(fma2(tk3[2], u, tk3[1]), u, tk3[0]);
+                            unpack2(fma2(k, t, nref), x[c], x[c + 1]);
+                        }
+                    } else if (degree == 5) {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            const f32x2 t = pack2(x[c], x[c + 1]), u = mul2(t, t);
                             f32x2 k = fma2(tk[4], u, tk[3]);
                             k = fma2(k, u, tk[2]);
                             k = fma2(k, u, tk[1]);
@@ -646,7 +670,7 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                 if (__all_sync(0xffffffffu, top <= g.small)) {
 #pragma unroll
                     for (int c = 0; c < kRows; c += 2) {
-                        const f32x2 t = mul2(pack2(z[c], z[c + 1]), sc), u = mul2(t, t);
+                        const f32x2 t = pack2(z[c], z[c + 1]), u = mul2(t, t);
                         f32x2 p = fma2(tk[4], u, tk[3]);
                         p = fma2(p, u, tk[2]);
                         p = fma2(p, u, tk[1]);
@@ -905,9 +929,16 @@ int masked_attention_launch(const AttentionShape& s, int nseg, uint64_t n_q, uin
     g.ldv = ldv;
     g.zscale = s.cap > 0.f ? 2.f * kLog2e * s.scale / s.cap : s.scale * kLog2e;
     g.zcap = s.cap * kLog2e;
-    g.tscale = s.cap > 0.f ? s.scale / s.cap : 0.f;
-    g.small = s.cap > 0.f ? kTanhLimit * s.cap / s.scale : 0.f;
-    for (int i = 0; i < 5; ++i) g.tanh[i] = kTanh[i] * g.zcap;
+    if (s.cap > 0.f) {
+        const double t = double(s.scale) / s.cap;
+        const bool fits = t <= kTanhScale && t * kTanhScale >= 1.0;
+        g.small = fits ? float(kTanhLimit / t) : -1.f;
+        double power = t * s.cap * 1.4426950408889634;
+        for (int i = 0; i < 5; ++i, power *= t * t) {
+            g.tanh[i] = fits ? float(kTanh[i] * power) : 0.f;
+            if (i < 3) g.tanh3[i] = fits ? float(kTanhShort[i] * power) : 0.f;
+        }
+    }
     g.out = static_cast<uint16_t*>(out);
     g.ldo = ldo;
     g.lse = lse;
