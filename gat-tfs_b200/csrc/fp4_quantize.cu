@@ -27,7 +27,6 @@ struct QuantArgs {
     int code_chunks; // of those, the ones inside the code row
     const void* x;
     int ldx;
-    int x_align;     // bytes to which every 8-column piece of x is aligned (at most 16)
     uint8_t* codes;
     int ldc;
     uint8_t* scales;
@@ -35,7 +34,7 @@ struct QuantArgs {
     float* row_scale;
     void* values;
     int ldv;
-    int v_align;
+    int v_bf16;
 };
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -43,23 +42,29 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 
 // 8 columns from element offset `off`, of which `valid` exist (zeros behind).
-template <bool BF16>
-__device__ __forceinline__ void load8(const QuantArgs& a, uint64_t off, int valid, float* v) {
+// VEC: fours of columns are whole and aligned.
+template <bool BF16, bool VEC>
+__device__ __forceinline__ void load8(const void* x, uint64_t off, int valid, float* v) {
     if constexpr (BF16) {
-        const uint16_t* p = static_cast<const uint16_t*>(a.x) + off;
-        uint32_t u[4];
-        if (valid == 8 && a.x_align >= 4) {
-            if (a.x_align >= 16) {
-                const uint4 t = ldg_nc_v4(p);
-                u[0] = t.x; u[1] = t.y; u[2] = t.z; u[3] = t.w;
-            } else if (a.x_align >= 8) {
-                const uint2 t0 = __ldg(reinterpret_cast<const uint2*>(p)), t1 = __ldg(reinterpret_cast<const uint2*>(p) + 1);
-                u[0] = t0.x; u[1] = t0.y; u[2] = t1.x; u[3] = t1.y;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) u[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+        const uint16_t* p = static_cast<const uint16_t*>(x) + off;
+        uint32_t u[4] = {0u, 0u, 0u, 0u};
+        if constexpr (VEC) {
+            if (valid > 0) {
+                const uint2 t = __ldg(reinterpret_cast<const uint2*>(p));
+                u[0] = t.x;
+                u[1] = t.y;
+            }
+            if (valid > 4) {
+                const uint2 t = __ldg(reinterpret_cast<const uint2*>(p) + 1);
+                u[2] = t.x;
+                u[3] = t.y;
             }
         } else {
 #pragma unroll
@@ -75,18 +80,44 @@ __device__ __forceinline__ void load8(const QuantArgs& a, uint64_t off, int vali
             v[2 * i + 1] = bf16hi(u[i]);
         }
     } else {
-        const float* p = static_cast<const float*>(a.x) + off;
-        if (valid == 8 && a.x_align >= 16) {
-            const float4 t0 = __ldg(reinterpret_cast<const float4*>(p)), t1 = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        const float* p = static_cast<const float*>(x) + off;
+        if constexpr (VEC) {
+            float4 t0 = make_float4(0.f, 0.f, 0.f, 0.f), t1 = t0;
+            if (valid > 0) t0 = __ldg(reinterpret_cast<const float4*>(p));
+            if (valid > 4) t1 = __ldg(reinterpret_cast<const float4*>(p) + 1);
             v[0] = t0.x; v[1] = t0.y; v[2] = t0.z; v[3] = t0.w;
             v[4] = t1.x; v[5] = t1.y; v[6] = t1.z; v[7] = t1.w;
-        } else if (valid == 4 && a.x_align >= 16) {
-            const float4 t0 = __ldg(reinterpret_cast<const float4*>(p));
-            v[0] = t0.x; v[1] = t0.y; v[2] = t0.z; v[3] = t0.w;
-            v[4] = v[5] = v[6] = v[7] = 0.f;
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = i < valid ? __ldg(p + i) : 0.f;
+        }
+    }
+}
+// The same for the values: y to element offset `off`.
+template <bool VEC>
+__device__ __forceinline__ void store8(void* out, bool bf16, uint64_t off, int valid, const float* y) {
+    if (bf16) {  // the values have at most six significant bits
+        uint16_t* p = static_cast<uint16_t*>(out) + off;
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(y[2 * i], y[2 * i + 1]);
+        if constexpr (VEC) {
+            if (valid > 0) reinterpret_cast<uint2*>(p)[0] = make_uint2(w[0], w[1]);
+            if (valid > 4) reinterpret_cast<uint2*>(p)[1] = make_uint2(w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < valid) p[i] = uint16_t(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
+        }
+    } else {
+        float* p = static_cast<float*>(out) + off;
+        if constexpr (VEC) {
+            if (valid > 0) reinterpret_cast<float4*>(p)[0] = make_float4(y[0], y[1], y[2], y[3]);
+            if (valid > 4) reinterpret_cast<float4*>(p)[1] = make_float4(y[4], y[5], y[6], y[7]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < valid) p[i] = y[i];
         }
     }
 }
@@ -144,17 +175,31 @@ __device__ __forceinline__ float row_power(float amax) {
     return __uint_as_float(uint32_t(j + 127) << 23);
 }
 
+// RN(1 / s) of an E4M3 number s > 0: one Newton step from an approximation
+// within an ulp or so; s has four significant bits, so no 1 / s lies near the
+// middle between two FP32 numbers.
+__device__ __forceinline__ float reciprocal_e4m3(float s) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(s));
+    return fmaf(y, fmaf(-s, y, 1.f), y);
+}
+
 // LANES lanes per row (16 or 32: part of a warp; 256: the CTA), CHUNKS pieces
 // of 8 columns a lane kept in registers. REREAD: rows longer than LANES *
-// CHUNKS * 8 columns are read a second time for the codes.
-template <int FORMAT, bool BF16, int LANES, int CHUNKS, bool REREAD>
+// CHUNKS * 8 columns are read a second time for the codes. VEC: width, rows of
+// x and rows of the values are whole, aligned fours of elements.
+// Issue slots bind it as much as memory does, hence packed FP32 pairs and no
+// branches on alignment inside: 2,449,029 x 100 FP32 to NVFP4 with BF16 values
+// took 389 us with scalar arithmetic and such branches and takes 294 us
+// (5.5 TB/s); 169,343 x 128 FP32 to MXFP4 25 us (5.6 TB/s).
+template <int FORMAT, bool BF16, bool VEC, int LANES, int CHUNKS, bool REREAD>
 __global__ void __launch_bounds__(256) fp4_quantize_kernel(const QuantArgs a) {
     constexpr bool kNv = FORMAT == GAT_B200_NVFP4;
     constexpr int kBlockLanes = fp4_block(FORMAT) / 8;  // lanes of one block
-    constexpr int kWordLanes = 4 * kBlockLanes;          // lanes of one scale word
     const int lane = threadIdx.x % LANES;
     const uint64_t row = LANES >= 256 ? uint64_t(blockIdx.x) : uint64_t(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
     const bool live = row < a.n;
+    const int width = live ? a.width : 0;
     const uint64_t xoff = row * uint64_t(a.ldx);
     float v[CHUNKS][8];
     float mine[CHUNKS];
@@ -163,20 +208,14 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(const QuantArgs a) {
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const int col = ((c0 + c) * LANES + lane) * 8;
-            const int valid = live ? min(8, a.width - col) : 0;
-            if (valid > 0) {
-                load8<BF16>(a, xoff + uint64_t(col), valid, v[c]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[c][i] = 0.f;
-            }
+            load8<BF16, VEC>(a.x, xoff + uint64_t(col), width - col, v[c]);
         }
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            float m = fabsf(v[c][0]);
-#pragma unroll
-            for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(v[c][i]));
-            mine[c] = m;
+            float m = max_nan(fabsf(v[c][0]), fabsf(v[c][1]), fabsf(v[c][2]));
+            m = max_nan(m, fabsf(v[c][3]), fabsf(v[c][4]));
+            m = max_nan(m, fabsf(v[c][5]), fabsf(v[c][6]));
+            mine[c] = max_nan(m, fabsf(v[c][7]));
         }
     };
 
@@ -204,14 +243,16 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(const QuantArgs a) {
         if (lane == 0 && live) a.row_scale[row] = r;
     }
     const bool row_nan = kNv && r != r;
+    uint8_t* code_row = a.codes + row * uint64_t(a.ldc);
+    uint8_t* scale_row = a.scales + (row >> 7) * uint64_t(a.tiles) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
 
     const int steps = REREAD || !kNv ? (a.chunks + LANES * CHUNKS - 1) / (LANES * CHUNKS) : 1;
     for (int s = 0; s < steps; ++s) {
         if (!kNv || REREAD) fetch(s * CHUNKS);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            const int chunk = (s * CHUNKS + c) * LANES + lane;
             if ((s * CHUNKS + c) * LANES >= a.chunks) break;  // the same for all lanes of the row
+            const int chunk = (s * CHUNKS + c) * LANES + lane;
             float m = mine[c];
 #pragma unroll
             for (int o = 1; o < kBlockLanes; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -225,67 +266,37 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(const QuantArgs a) {
                 byte = row_nan ? 0u : to_e4m3(q);
                 const float sc = from_e4m3(byte);
                 d = sc * r;
-                inv = sc > 0.f ? __frcp_rn(sc) * rinv : 0.f;
+                inv = sc > 0.f ? reciprocal_e4m3(sc) * rinv : 0.f;
             } else {
                 const uint32_t u = __float_as_uint(m);
                 const int e = int(u >> 23) - 2;  // biased exponent of the scale
-                byte = u >= 0x7f800000u ? 255u : (e > 0 ? uint32_t(e) : 0u);
-                d = byte == 255u ? __uint_as_float(0x7fc00000u)
-                                 : (byte ? __uint_as_float(byte << 23) : __uint_as_float(0x400000u));
+                byte = u >= 0x7f800000u ? 255u : uint32_t(max(e, 0));
+                d = byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte ? byte << 23 : 0x400000u);
                 inv = byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
             }
             float q[8];
+            const f32x2 inv2 = pack2(inv, inv), nd2 = pack2(-d, -d);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                q[i] = v[c][i] * inv;
-                if constexpr (kNv) q[i] = fmaf(fmaf(-q[i], d, v[c][i]), inv, q[i]);
+            for (int i = 0; i < 8; i += 2) {
+                const f32x2 x2 = pack2(v[c][i], v[c][i + 1]);
+                f32x2 q2 = mul2(x2, inv2);
+                if constexpr (kNv) q2 = fma2(fma2(q2, nd2, x2), inv2, q2);
+                unpack2(q2, q[i], q[i + 1]);
             }
-            uint32_t code = e2m1x8(q);
-            if (inv == 0.f) code = 0;
-            // the four scale bytes of a word, in the lane of its first block
-            uint32_t word = byte;
-            word |= __shfl_down_sync(0xffffffffu, byte, kBlockLanes) << 8;
-            word |= __shfl_down_sync(0xffffffffu, byte, 2 * kBlockLanes) << 16;
-            word |= __shfl_down_sync(0xffffffffu, byte, 3 * kBlockLanes) << 24;
+            const uint32_t code = inv == 0.f ? 0u : e2m1x8(q);
             if (!live || chunk >= a.chunks) continue;
-            if (chunk < a.code_chunks)
-                *reinterpret_cast<uint32_t*>(a.codes + row * uint64_t(a.ldc) + uint64_t(chunk) * 4) = code;
-            if (chunk % kWordLanes == 0)
-                *reinterpret_cast<uint32_t*>(a.scales + ((row >> 7) * uint64_t(a.tiles) + chunk / kWordLanes) * 512 +
-                                             (row & 31) * 16 + ((row >> 5) & 3) * 4) = word;
-            const int valid = min(8, a.width - chunk * 8);
-            if (a.values && valid > 0) {
+            if (chunk < a.code_chunks) *reinterpret_cast<uint32_t*>(code_row + uint32_t(chunk) * 4) = code;
+            if (lane % kBlockLanes == 0) {
+                const uint32_t block = uint32_t(chunk) / kBlockLanes;
+                scale_row[uint64_t(block >> 2) * 512 + (block & 3)] = uint8_t(byte);
+            }
+            if (a.values) {
                 float y[8];
                 from_e2m1x8(code, y);
+                const f32x2 d2 = pack2(d, d);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] *= d;
-                const uint64_t off = row * uint64_t(a.ldv) + uint64_t(chunk) * 8;
-                if (a.v_align < 0) {  // FP32 values
-                    float* p = static_cast<float*>(a.values) + off;
-                    if (valid == 8 && a.v_align <= -16) {
-                        reinterpret_cast<float4*>(p)[0] = make_float4(y[0], y[1], y[2], y[3]);
-                        reinterpret_cast<float4*>(p)[1] = make_float4(y[4], y[5], y[6], y[7]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (i < valid) p[i] = y[i];
-                    }
-                } else {  // BF16: the values have at most six significant bits
-                    uint16_t* p = static_cast<uint16_t*>(a.values) + off;
-                    uint32_t w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(y[2 * i], y[2 * i + 1]);
-                    if (valid == 8 && a.v_align >= 16) {
-                        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-                    } else if (a.v_align >= 8 && (valid & 3) == 0) {
-                        reinterpret_cast<uint2*>(p)[0] = make_uint2(w[0], w[1]);
-                        if (valid == 8) reinterpret_cast<uint2*>(p)[1] = make_uint2(w[2], w[3]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (i < valid) p[i] = uint16_t(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
-                    }
-                }
+                for (int i = 0; i < 8; i += 2) unpack2(mul2(pack2(y[i], y[i + 1]), d2), y[i], y[i + 1]);
+                store8<VEC>(a.values, a.v_bf16, row * uint64_t(a.ldv) + uint64_t(chunk) * 8, width - chunk * 8, y);
             }
         }
     }
@@ -297,29 +308,34 @@ int row_align(const void* base, uint64_t pitch) {
     return int(u & (~u + 1));
 }
 
-template <int FORMAT, bool BF16>
+template <int FORMAT, bool BF16, bool VEC>
 int launch_quantize(const QuantArgs& a, cudaStream_t st) {
     // 16 or 32 lanes a row while a row fits them once, one warp up to 1024
-    // columns, the CTA for longer ones; above 16384 columns NVFP4 reads twice.
-    const uint64_t per16 = (a.n + 15) / 16, per8 = (a.n + 7) / 8;
+    // columns, the CTA for longer ones; above 8192 columns NVFP4 reads twice.
+    const unsigned per16 = unsigned((a.n + 15) / 16), per8 = unsigned((a.n + 7) / 8), n = unsigned(a.n);
     if (a.chunks <= 16)
-        fp4_quantize_kernel<FORMAT, BF16, 16, 1, false><<<unsigned(per16), 256, 0, st>>>(a);
+        fp4_quantize_kernel<FORMAT, BF16, VEC, 16, 1, false><<<per16, 256, 0, st>>>(a);
     else if (a.chunks <= 32)
-        fp4_quantize_kernel<FORMAT, BF16, 32, 1, false><<<unsigned(per8), 256, 0, st>>>(a);
+        fp4_quantize_kernel<FORMAT, BF16, VEC, 32, 1, false><<<per8, 256, 0, st>>>(a);
     else if (a.chunks <= 64)
-        fp4_quantize_kernel<FORMAT, BF16, 32, 2, false><<<unsigned(per8), 256, 0, st>>>(a);
+        fp4_quantize_kernel<FORMAT, BF16, VEC, 32, 2, false><<<per8, 256, 0, st>>>(a);
     else if (a.chunks <= 128)
-        fp4_quantize_kernel<FORMAT, BF16, 32, 4, false><<<unsigned(per8), 256, 0, st>>>(a);
+        fp4_quantize_kernel<FORMAT, BF16, VEC, 32, 4, false><<<per8, 256, 0, st>>>(a);
     else if (a.chunks <= 256)
-        fp4_quantize_kernel<FORMAT, BF16, 256, 1, false><<<unsigned(a.n), 256, 0, st>>>(a);
+        fp4_quantize_kernel<FORMAT, BF16, VEC, 256, 1, false><<<n, 256, 0, st>>>(a);
     else if (a.chunks <= 512)
-        fp4_quantize_kernel<FORMAT, BF16, 256, 2, false><<<unsigned(a.n), 256, 0, st>>>(a);
+        fp4_quantize_kernel<FORMAT, BF16, VEC, 256, 2, false><<<n, 256, 0, st>>>(a);
     else if (a.chunks <= 1024)
-        fp4_quantize_kernel<FORMAT, BF16, 256, 4, false><<<unsigned(a.n), 256, 0, st>>>(a);
+        fp4_quantize_kernel<FORMAT, BF16, VEC, 256, 4, false><<<n, 256, 0, st>>>(a);
     else
-        fp4_quantize_kernel<FORMAT, BF16, 256, 4, true><<<unsigned(a.n), 256, 0, st>>>(a);
+        fp4_quantize_kernel<FORMAT, BF16, VEC, 256, 4, true><<<n, 256, 0, st>>>(a);
     GATB_LAUNCH("fp4_quantize kernel");
     return 0;
+}
+template <int FORMAT>
+int launch_quantize(const QuantArgs& a, bool bf16, bool vec, cudaStream_t st) {
+    if (bf16) return vec ? launch_quantize<FORMAT, true, true>(a, st) : launch_quantize<FORMAT, true, false>(a, st);
+    return vec ? launch_quantize<FORMAT, false, true>(a, st) : launch_quantize<FORMAT, false, false>(a, st);
 }
 
 }  // namespace
@@ -357,19 +373,18 @@ int fp4_quantize_launch(int format, uint64_t n, int width, const void* x, int x_
     a.code_chunks = fp4_row_bytes(width) / 4;
     a.x = x;
     a.ldx = ldx;
-    a.x_align = row_align(x, uint64_t(ldx) * xs);
     a.codes = static_cast<uint8_t*>(codes);
     a.ldc = ldc;
     a.scales = static_cast<uint8_t*>(scales);
     a.row_scale = row_scale;
     a.values = values;
     a.ldv = ldv;
-    a.v_align = values ? row_align(values, uint64_t(ldv) * vs) * (v_dtype == GAT_B200_F32 ? -1 : 1) : 0;
-    if (format == GAT_B200_MXFP4)
-        return x_dtype == GAT_B200_BF16 ? launch_quantize<GAT_B200_MXFP4, true>(a, st)
-                                        : launch_quantize<GAT_B200_MXFP4, false>(a, st);
-    return x_dtype == GAT_B200_BF16 ? launch_quantize<GAT_B200_NVFP4, true>(a, st)
-                                    : launch_quantize<GAT_B200_NVFP4, false>(a, st);
+    a.v_bf16 = v_dtype == GAT_B200_BF16;
+    const bool vec = width % 4 == 0 && row_align(x, uint64_t(ldx) * xs) >= 4 * xs &&
+                     (!values || row_align(values, uint64_t(ldv) * vs) >= 4 * vs);
+    const bool bf16 = x_dtype == GAT_B200_BF16;
+    return format == GAT_B200_MXFP4 ? launch_quantize<GAT_B200_MXFP4>(a, bf16, vec, st)
+                                    : launch_quantize<GAT_B200_NVFP4>(a, bf16, vec, st);
 }
 
 }  // namespace gatb

@@ -184,7 +184,10 @@ def _ptr(t) -> Optional[int]:
 def _stream(s) -> Optional[int]:
     if s is None:
         return None
-    return s.cuda_stream if hasattr(s, "cuda_stream") else int(s)
+    try:
+        return s.cuda_stream
+    except AttributeError:
+        return int(s)
 
 
 def version() -> int:
