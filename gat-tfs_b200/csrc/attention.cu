@@ -60,7 +60,7 @@ struct AttnArgs {
     const float* slopes;
     const uint16_t* v;
     int ldv;
-    float zscale;    // without a cap: scale * log2 e; with one: 2 log2 e * scale / cap
+    float zscale;    // without a cap: scale * log2 e; with one: scale / cap
     float zcap;      // cap * log2 e
     float small;     // raw scores up to which the tanh's long polynomial holds (half of it: the short one)
     float tanh[5];   // coefficients of s, s^3 .. in zcap tanh(scale / cap * s)
@@ -167,15 +167,11 @@ __device__ __forceinline__ uint32_t visible(int b, int e) {
 constexpr float kGrow = 24.f;
 // Largest cap * log2 e whose weights are taken relative to half of it.
 constexpr float kFixedCap = 80.f;
-// tanh(x) = x p(x^2), minimax polynomials (Remez exchange): five terms for
-// |x| <= 0.6, relative error 7.4e-8, and three for |x| <= 0.3, 1.2e-6 (of a
-// score of at most 0.3 cap: 2.5e-5 in a weight's exponent at the very end).
-constexpr float kTanhLimit = 0.6f;
-constexpr float kTanh[5] = {0.999999926872f, -0.333323099889f, 0.133101737673f, -0.0521014822761f, 0.0154754278422f};
-constexpr float kTanhShort[3] = {0.99999883885f, -0.33310021606f, 0.126339459906f};
-// The coefficients take scale / cap into themselves, in powers up to the ninth:
-// outside this range of it the tanh is computed from exponentials.
-constexpr float kTanhScale = 8192.f;
+// The polynomials' coefficients take scale / cap into themselves, in powers up
+// to the ninth: used for scale / cap up to kTanhScale and products q.k whose
+// powers stay FP32 numbers; other scores go one by one through capped_score().
+constexpr double kTanhScale = 8192.0;
+constexpr float kTanhProducts = 4915.f;
 
 // DP: dim rounded up to 64 or 128. CAP / BIAS: scores go through the tanh / get the distance bias.
 // FIXED: weights relative to half the cap (capped scores without a bias).
@@ -601,7 +597,7 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                         }
                     } else {
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) x[c] = fmaf(g.zcap, tanh_of_log2(x[c] * g.zscale), -m);
+                        for (int c = 0; c < 32; ++c) x[c] = capped_score(x[c] * g.zscale, g.zcap) - m;
                     }
                     if (sw == 1) {
                         const uint32_t bits = visible(jl - 32 * w, jh - 32 * w);
@@ -647,7 +643,7 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                     }
                 } else {
 #pragma unroll
-                    for (int c = 0; c < kRows; ++c) z[c] = g.zcap * tanh_of_log2(z[c] * g.zscale);
+                    for (int c = 0; c < kRows; ++c) z[c] = capped_score(z[c] * g.zscale, g.zcap);
                 }
             }
             if constexpr (BIAS) {
@@ -856,8 +852,9 @@ int attention_check(const char* what, const AttentionShape& s, uint64_t n_q, uin
     if (s.dim <= 0 || s.dim > 128 || s.dim % 8) return fail_code(GAT_B200_EUNSUPPORTED, w + "dim must be a multiple of 8, at most 128");
     if (n_q > uint64_t(INT32_MAX - 512) || n_k > uint64_t(INT32_MAX - 512)) return fail(w + "too many rows");
     if (nseg < 0) return fail(w + "bad segment count");
-    if (!(s.scale > 0.f) || !(s.scale < 3e38f)) return fail(w + "scale must be positive and finite");
-    if (!(s.cap >= 0.f) || !(s.cap < 3e38f)) return fail(w + "cap must be finite and not negative (0: none)");
+    if (!(s.scale > 0.f) || s.scale > 1e30f) return fail(w + "scale must be positive, at most 1e30");
+    if (!(s.cap >= 0.f) || s.cap > 1e30f) return fail(w + "cap must lie in 0 (none) .. 1e30");
+    if (s.cap > 0.f && s.scale / s.cap > 1e30f) return fail(w + "cap too small for the scale");
     const int64_t hq = int64_t(s.heads) * s.dim, hk = int64_t(s.kv_heads) * s.dim;
     if (ldq < hq || ldk < hk || ldv < hk || ldo < hq) return fail(w + "row stride smaller than heads * dim");
     if ((ldq | ldk | ldv | ldo) % 8) return fail(w + "rows must be 16-byte aligned");
@@ -895,12 +892,12 @@ int masked_attention_launch(const AttentionShape& s, int nseg, uint64_t n_q, uin
     g.slopes = s.slopes;
     g.v = static_cast<const uint16_t*>(v);
     g.ldv = ldv;
-    g.zscale = s.cap > 0.f ? 2.f * kLog2e * s.scale / s.cap : s.scale * kLog2e;
+    g.zscale = s.cap > 0.f ? s.scale / s.cap : s.scale * kLog2e;
     g.zcap = s.cap * kLog2e;
     if (s.cap > 0.f) {
         const double t = double(s.scale) / s.cap;
-        const bool fits = t <= kTanhScale && t * kTanhScale >= 1.0;
-        g.small = fits ? float(kTanhLimit / t) : -1.f;
+        const bool fits = t <= kTanhScale;
+        g.small = !fits ? -1.f : kTanhLimit / t < kTanhProducts ? float(kTanhLimit / t) : kTanhProducts;
         double power = t * s.cap * 1.4426950408889634;
         for (int i = 0; i < 5; ++i, power *= t * t) {
             g.tanh[i] = fits ? float(kTanh[i] * power) : 0.f;

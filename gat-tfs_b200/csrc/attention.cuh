@@ -23,6 +23,23 @@ __device__ __forceinline__ float rcp(float x) {
 // the whole range (2^x = inf gives 1, 2^x = 0 gives -1).
 __device__ __forceinline__ float tanh_of_log2(float x) { return fmaf(-2.f, rcp(ex2(x) + 1.f), 1.f); }
 
+// tanh(x) = x p(x^2), minimax polynomials (Remez exchange): five terms for
+// |x| <= 0.6, relative error 7.4e-8, and three for |x| <= 0.3, 1.2e-6 (of a
+// score of at most 0.3 cap).
+constexpr float kTanhLimit = 0.6f;
+constexpr float kTanh[5] = {0.999999926872f, -0.333323099889f, 0.133101737673f, -0.0521014822761f, 0.0154754278422f};
+constexpr float kTanhShort[3] = {0.99999883885f, -0.33310021606f, 0.126339459906f};
+// cap log2 e tanh(t), t = scale s / cap, for any cap and score: where tanh(t)
+// is small against 1 the exponentials would cancel.
+__device__ __forceinline__ float capped_score(float t, float zcap) {
+    const float u = t * t;
+    float p = fmaf(0.0154754278422f, u, -0.0521014822761f);
+    p = fmaf(p, u, 0.133101737673f);
+    p = fmaf(p, u, -0.333323099889f);
+    p = fmaf(p, u, 0.999999926872f);
+    return zcap * (fabsf(t) <= kTanhLimit ? t * p : tanh_of_log2(t * (2.f * kLog2e)));
+}
+
 // What attention_check() settles for both kernels.
 struct AttentionShape {
     int heads, kv_heads, dim;

@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_step_kernel(const StepA
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         float& x = z[t][2 * h + i];
-                        x = CAP ? a.zcap * tanh_of_log2(x * a.zscale) : x * a.zscale;
+                        x = CAP ? capped_score(x * a.zscale, a.zcap) : x * a.zscale;
                         if constexpr (BIAS) x = fmaf(slope[i], float(len - 1 - (j + key)), x);
                         if (key >= left) x = -INFINITY;
                         mb[i] = fmaxf(mb[i], x);
@@ -466,7 +466,7 @@ int masked_attention_step_launch(const AttentionShape& s, int nseg, uint64_t n_k
     a.ldq = ldq;
     a.ldk = ldk;
     a.ldv = ldv;
-    a.zscale = s.cap > 0.f ? 2.f * kLog2e * s.scale / s.cap : s.scale * kLog2e;
+    a.zscale = s.cap > 0.f ? s.scale / s.cap : s.scale * kLog2e;
     a.zcap = s.cap * kLog2e;
     a.out = static_cast<uint16_t*>(out);
     a.ldo = ldo;

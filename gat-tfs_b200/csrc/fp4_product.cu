@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             rb[lane + 32] = rb1;
             __syncwarp();
             if (t + pairs < ntiles) fetch(t + pairs);
-            if (!mbar_wait(acc_full + odd, (tl >> 1) & 1u, abort_flag, &g_fp4_error)) break;
+            if (!mbar_wait_warp(acc_full + odd, (tl >> 1) & 1u, abort_flag, &g_fp4_error)) break;
             fence_after();
             float v[64];
             tmem_ld64(tmem + (odd ? kOdd : 0) + (uint32_t(q * 32) << 16) + grp * 64, v);

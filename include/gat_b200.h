@@ -363,7 +363,8 @@ int gat_b200_aggregate_fused_noalloc(uint64_t n, uint64_t e, const uint64_t* row
  * q, out: BF16 [n_q][heads * dim]; k, v: BF16 [n_k][kv_heads * dim]; query head
  * h reads key head h / (heads / kv_heads). ld* are row strides in elements;
  * rows 16-byte aligned. lse: FP32 [n_q][heads] or NULL. slopes: FP32 [heads].
- * dim: a multiple of 8, at most 128 (GAT_B200_EUNSUPPORTED otherwise). Scores
+ * dim: a multiple of 8, at most 128 (GAT_B200_EUNSUPPORTED otherwise). scale in
+ * (0, 1e30], cap in [0, 1e30]. Scores
  * and sums are FP32; the weights are rounded to BF16 for the second product. */
 int gat_b200_masked_attention(int heads, int kv_heads, int dim, int nseg, uint64_t n_q, uint64_t n_k,
                               const uint64_t* q_row, const uint64_t* k_row, int mask,

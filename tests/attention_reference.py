@@ -36,13 +36,14 @@ def attention(q, k, v, q_row, k_row, heads, kv_heads, dim, scale, cap=0.0, slope
             c = v[k0:k1, g * dim:(g + 1) * dim].double()
             dot = a @ b.t() * scale
             z = cap * torch.tanh(dot / cap) if cap > 0 else dot
-            # FP32: dim products and sums of the dot, then a handful of roundings of values up to z's size
-            err = (a.abs() @ b.abs().t()) * scale * (dim + 4) * 2.0 ** -24 + (cap if cap > 0 else 0) * 2.0 ** -20
+            # FP32: dim products and sums of the dot, then a handful of roundings of values up to z's size; a
+            # tanh within 1.3e-6 < 2^-19 of itself (tanh' <= 1: the dot's error grows no further)
+            err = (a.abs() @ b.abs().t()) * scale * (dim + 4) * 2.0 ** -24
             if slopes is not None:
                 far = (pos[:, None] - key[None, :]).abs().double()
                 z = z - slopes[h].double() * far
                 err = err + slopes[h].double() * far * 2.0 ** -21
-            err = err + z.abs() * 2.0 ** -21 + 2.0 ** -20
+            err = err + z.abs() * 2.0 ** (-19 if cap > 0 else -21) + 2.0 ** -20
             z = torch.where(seen, z, torch.full_like(z, -math.inf))
             err = torch.where(seen, err, torch.zeros_like(err))
             top = z.amax(1, keepdim=True)

@@ -17,6 +17,9 @@ COMMON = [
     (dict(scale=INF), "scale", G.EINVAL),
     (dict(cap=-1.0), "cap", G.EINVAL),
     (dict(cap=INF), "cap", G.EINVAL),
+    (dict(cap=2e30), "cap", G.EINVAL),
+    (dict(cap=1e-35), "cap too small", G.EINVAL),
+    (dict(scale=2e30), "scale", G.EINVAL),
     (dict(ldq=100), "row stride", G.EINVAL),
     (dict(ldo=124), "row stride", G.EINVAL),
     (dict(ldk=63), "row stride", G.EINVAL),

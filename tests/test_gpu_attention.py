@@ -153,6 +153,21 @@ def test_large_scores(G, dev):
             b.check(b.reference(mask=mask, cap=cap))
 
 
+@pytest.mark.parametrize("cap", [1e-4, 0.3, 5.0, 56.0, 1000.0, 1e6, 1e20])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_caps_far_from_the_scores(G, dev, cap, dim):
+    # caps that all scores exceed, caps that no score comes near, and both sides of the polynomials' ranges
+    lens = [300, 150]
+    for bias in (False, True):
+        sl = slopes_of(2, dev) if bias else None
+        b = Batch(dev, lens, lens, 2, 1, dim, seed=4, qscale=6.0)
+        b.run(G, 1, None, cap, sl)
+        b.check(b.reference(mask=1, cap=cap, slopes=sl))
+        s = Step(dev, lens, 2, 1, dim, seed=4)
+        s.run_step(G, cap, sl)
+        s.check(s.want(cap=cap, slopes=sl))
+
+
 def test_fused_table_and_streams(G, dev):
     """Q, K and V as column ranges of one projection's output, on a stream of its own."""
     heads, kv, dim, n = 4, 2, 32, 333
