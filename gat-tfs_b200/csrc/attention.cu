@@ -27,12 +27,13 @@
 // the sum keeps the unrounded FP32 weights).
 // The exponentials bound it (16 a clock and SM; a 128 x 128 block of dim 128
 // takes the tensor cores as long as its exponentials): the cap's tanh is a
-// polynomial on the FMA pipe wherever a block's scores stay below 0.6 cap. Capped
-// scores without a bias lie within +-cap, so up to a cap of 55 their weights
-// are taken relative to cap / 2 instead of the running maximum (2^-120 .. 2^40
-// and their sums are ordinary FP32 and BF16 numbers): no pass for the maximum,
-// no rescaling, 32 columns at a time flow from S to P and two threads share a
-// row. (With a maximum to agree on, two threads a row were slower than one.)
+// polynomial on the FMA pipe wherever a block's scores stay below 0.6 cap. A
+// row's largest capped score lies within +-cap (of the bias of its nearest key),
+// so up to a cap of 55 the weights are taken relative to cap / 2 (and that bias)
+// instead of the running maximum (the largest is 2^-120 .. 2^40, an ordinary FP32
+// and BF16 number): no pass for the maximum, no rescaling, 32 columns at a time
+// flow from S to P and two threads share a row. (With a maximum to agree on, two
+// threads a row were slower than one: 8192 x 32 x 128 causal, 320 us and 359 us.)
 #include <cuda.h>
 
 #include "attention.cuh"
@@ -174,7 +175,7 @@ constexpr double kTanhScale = 8192.0;
 constexpr float kTanhProducts = 4915.f;
 
 // DP: dim rounded up to 64 or 128. CAP / BIAS: scores go through the tanh / get the distance bias.
-// FIXED: weights relative to half the cap (capped scores without a bias).
+// FIXED: weights relative to half the cap (capped scores).
 // TMEM, one tile: S at 0, P at 128, O at 192; two: S and P of tile t at 128 t, O at 256 + 128 t.
 template <int DP, bool FIXED>
 struct Shape {
@@ -197,7 +198,7 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
     attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnArgs g) {
     constexpr int kTiles = Shape<DP, FIXED>::kTiles, kHalves = Shape<DP, FIXED>::kHalves, kTile = Shape<DP, FIXED>::kTile, kSt = Shape<DP, FIXED>::kStages;
-    static_assert(!FIXED || (CAP && !BIAS), "only capped scores are bounded");
+    static_assert(!FIXED || CAP, "only capped scores are bounded");
     constexpr bool kOwnP = kTiles == 1;
     // P's columns for the block's keys 64 and up start kPHalf behind the others: where P overlays S, each
     // half of P lies in its own half of S
@@ -507,10 +508,16 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
 #pragma unroll
             for (int i = 0; i < 5; ++i) tk[i] = pack2(g.tanh[i], g.tanh[i]);
 #pragma unroll
-            for (int i = 0; i < 3; ++i) tk3[i] = pair_of(g.tanh3[i]);
+            for (int i = 0; i < 3; ++i) tk3[i] = FIXED ? pair_of(g.tanh3[i]) : 0;
         }
         // the reference maximum (log2 units) and the sum of the weights
         float m = FIXED ? 0.5f * g.zcap : -INFINITY, l = 0.f;
+        // FIXED with a bias: the distance of the row's nearest key (farthest with a negative slope), whose
+        // bias the weights are relative to
+        const int past = pos - (hi - lo - 1);  // behind the last key that it sees
+        const float near = !FIXED || !BIAS ? 0.f
+                           : nslope <= 0.f ? float(max(0, max(-pos, past)))
+                                           : fmaxf(fabsf(float(pos)), fabsf(float(past)));
         // the intervals of the warp's rows that see anything: smallest and largest begin and end
         const bool some = hi > lo;
         const int lo_min = __reduce_min_sync(0xffffffffu, some ? lo : INT32_MAX);
@@ -548,7 +555,6 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
             };
             if constexpr (FIXED) {
                 f32x2 sum = pack2(0.f, 0.f), sum2 = sum;
-                const f32x2 nref = pack2(-m, -m);
                 if (!p_is_free()) { ok = false; break; }
                 float x2[2][32];
                 tmem_ld32_start(s_t + 64 * half, x2[0]);
@@ -578,6 +584,10 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                         tmem_st16(p_t + kPHalf * half + 16 * i, p);
                         continue;
                     }
+                    const float rel = float(pos + jl - 32 * w);  // distance of column c: |rel - c|
+                    const bool before = BIAS && __all_sync(0xffffffffu, rel >= 31.f);
+                    const float off = before ? fmaf(nslope, rel - near, -m) : -m;
+                    const f32x2 nref = pack2(off, off);
                     if (degree == 3) {
 #pragma unroll
                         for (int c = 0; c < 32; c += 2) {
@@ -597,7 +607,14 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                         }
                     } else {
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) x[c] = capped_score(x[c] * g.zscale, g.zcap) - m;
+                        for (int c = 0; c < 32; ++c) x[c] = capped_score(x[c] * g.zscale, g.zcap) + off;
+                    }
+                    if (before) {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) x[c] = fmaf(float(-c), nslope, x[c]);
+                    } else if (BIAS) {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) x[c] = fmaf(nslope, fabsf(rel - float(c)) - near, x[c]);
                     }
                     if (sw == 1) {
                         const uint32_t bits = visible(jl - 32 * w, jh - 32 * w);
@@ -648,18 +665,19 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
             }
             if constexpr (BIAS) {
                 const float rel = float(pos + jl);  // distance of column c: |rel - c|
-                if (__all_sync(0xffffffffu, rel >= float(kRows - 1))) {
+                // (with a cap as well there are no registers to spare for the shorter form)
+                if (!CAP && __all_sync(0xffffffffu, rel >= float(kRows - 1))) {
                     const float base = nslope * rel;
 #pragma unroll
                     for (int c = 0; c < kRows; ++c) {
                         const float e = fmaf(float(-c), nslope, base);
-                        z[c] = CAP ? z[c] + e : fmaf(z[c], g.zscale, e);
+                        z[c] = fmaf(z[c], g.zscale, e);
                     }
                 } else {
 #pragma unroll
                     for (int c = 0; c < kRows; ++c) {
-                        const float e = nslope * fabsf(rel - float(c));
-                        z[c] = CAP ? z[c] + e : fmaf(z[c], g.zscale, e);
+                        if constexpr (!CAP) z[c] *= g.zscale;
+                        z[c] = fmaf(nslope, fabsf(rel - float(c)), z[c]);
                     }
                 }
             }
@@ -799,7 +817,7 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                 }
                 __syncwarp();
             }
-            if (live && g.lse && half == 0) g.lse[row * g.heads + head] = hi > lo ? (m + log2f(l)) * kLn2 : -INFINITY;
+            if (live && g.lse && half == 0) g.lse[row * g.heads + head] = hi > lo ? ((FIXED && BIAS ? fmaf(nslope, near, m) : m) + log2f(l)) * kLn2 : -INFINITY;
         }
     }
     if (my_to == 0 && row < g.n_q && half == 0) {  // every row of the tile sees nothing
@@ -837,7 +855,8 @@ int launch(const AttnArgs& g, const CUtensorMap& q, const CUtensorMap& k, const 
 template <int DP>
 int launch(const AttnArgs& g, bool cap, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
            cudaStream_t st) {
-    if (cap && !g.slopes && g.zcap <= kFixedCap) return launch<DP, true, false, true>(g, q, k, v, st);
+    if (cap && g.zcap <= kFixedCap)
+        return g.slopes ? launch<DP, true, true, true>(g, q, k, v, st) : launch<DP, true, false, true>(g, q, k, v, st);
     if (cap) return g.slopes ? launch<DP, true, true, false>(g, q, k, v, st) : launch<DP, true, false, false>(g, q, k, v, st);
     return g.slopes ? launch<DP, false, true, false>(g, q, k, v, st) : launch<DP, false, false, false>(g, q, k, v, st);
 }

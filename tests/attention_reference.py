@@ -42,7 +42,7 @@ def attention(q, k, v, q_row, k_row, heads, kv_heads, dim, scale, cap=0.0, slope
             if slopes is not None:
                 far = (pos[:, None] - key[None, :]).abs().double()
                 z = z - slopes[h].double() * far
-                err = err + slopes[h].double() * far * 2.0 ** -21
+                err = err + slopes[h].double().abs() * far * 2.0 ** -21
             err = err + z.abs() * 2.0 ** (-19 if cap > 0 else -21) + 2.0 ** -20
             z = torch.where(seen, z, torch.full_like(z, -math.inf))
             err = torch.where(seen, err, torch.zeros_like(err))

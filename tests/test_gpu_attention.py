@@ -153,6 +153,21 @@ def test_large_scores(G, dev):
             b.check(b.reference(mask=mask, cap=cap))
 
 
+@pytest.mark.parametrize("cap", [0.0, 20.0, 60.0])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("mask", [0, 1, 2])
+def test_slopes_of_either_sign(G, dev, cap, dim, mask):
+    sl = torch.tensor([1.5, -0.75, 0.0, -2.0], device=dev)
+    for q_lens, k_lens in (([400, 30, 1], [400, 30, 1]), ([40, 300], [700, 20])):
+        b = Batch(dev, q_lens, k_lens, 4, 2, dim, seed=9)
+        prefix = [n // 2 for n in k_lens] if mask == 2 else None
+        b.run(G, mask, prefix, cap, sl)
+        b.check(b.reference(mask=mask, prefix=prefix, cap=cap, slopes=sl))
+    s = Step(dev, [700, 1, 33], 4, 2, dim, seed=2)
+    s.run_step(G, cap, sl)
+    s.check(s.want(cap=cap, slopes=sl))
+
+
 @pytest.mark.parametrize("cap", [1e-4, 0.3, 5.0, 56.0, 1000.0, 1e6, 1e20])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_caps_far_from_the_scores(G, dev, cap, dim):
