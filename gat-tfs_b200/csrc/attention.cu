@@ -157,6 +157,23 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
+// Sums of weights and of their BF16 roundings.
+struct WeightSum {
+    f32x2 w[2], r[2];
+    __device__ __forceinline__ WeightSum() { w[0] = w[1] = r[0] = r[1] = pack2(0.f, 0.f); }
+    __device__ __forceinline__ void add(int i, float p0, float p1, uint32_t rounded) {
+        w[i & 1] = add2(w[i & 1], pack2(p0, p1));
+        r[i & 1] = add2(r[i & 1], pack2(bf16lo(rounded), bf16hi(rounded)));
+    }
+    __device__ __forceinline__ void into(float& sum, float& sum_rounded) const {
+        float a, b;
+        unpack2(add2(w[0], w[1]), a, b);
+        sum += a + b;
+        unpack2(add2(r[0], r[1]), a, b);
+        sum_rounded += a + b;
+    }
+};
+
 // Bits of the columns [b, e) of 32.
 __device__ __forceinline__ uint32_t visible(int b, int e) {
     b = min(max(b, 0), 32);
@@ -191,7 +208,7 @@ struct Shape {
     static constexpr int kTmem = DP == 64 ? 256 : 512;
     static constexpr int kTile = kRows * DP * 2;         // bytes of a Q tile, a K block, a V block
     static constexpr int kStages = 2;                    // K and V stages
-    static constexpr int kSmem = (kTiles + 2 * kStages) * kTile + (FIXED ? kTiles * 2 * kRows * 4 : 0) + 1024 + 512;
+    static constexpr int kSmem = (kTiles + 2 * kStages) * kTile + (FIXED ? kTiles * 4 * kRows * 4 : 0) + 1024 + 512;
 };
 template <int DP, bool CAP, bool BIAS, bool FIXED>
 __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::kCtas)
@@ -208,8 +225,8 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
     uint8_t* q_s = smem;
     uint8_t* k_s = q_s + kTiles * kTile;
     uint8_t* v_s = k_s + kSt * kTile;
-    float* sums = reinterpret_cast<float*>(v_s + kSt * kTile);  // FIXED: [kTiles][2][kRows]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sums + (FIXED ? kTiles * 2 * kRows : 0));
+    float* sums = reinterpret_cast<float*>(v_s + kSt * kTile);  // FIXED: [kTiles][4][kRows]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sums + (FIXED ? kTiles * 4 * kRows : 0));
     uint64_t* q_full = bars;
     uint64_t* k_full = bars + 1;
     uint64_t* k_empty = k_full + kSt;
@@ -510,8 +527,8 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
 #pragma unroll
             for (int i = 0; i < 3; ++i) tk3[i] = FIXED ? pair_of(g.tanh3[i]) : 0;
         }
-        // the reference maximum (log2 units) and the sum of the weights
-        float m = FIXED ? 0.5f * g.zcap : -INFINITY, l = 0.f;
+        // the reference maximum (log2 units), the sums of the weights and of the rounded weights
+        float m = FIXED ? 0.5f * g.zcap : -INFINITY, l = 0.f, lr = 0.f;
         // FIXED with a bias: the distance of the row's nearest key (farthest with a negative slope), whose
         // bias the weights are relative to
         const int past = pos - (hi - lo - 1);  // behind the last key that it sees
@@ -554,7 +571,7 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                 return !kOwnP || use == 0 || mbar_wait_warp(pv_done, (use - 1) & 1u, abort_flag, &g_attention_error);
             };
             if constexpr (FIXED) {
-                f32x2 sum = pack2(0.f, 0.f), sum2 = sum;
+                WeightSum sum;
                 if (!p_is_free()) { ok = false; break; }
                 float x2[2][32];
                 tmem_ld32_start(s_t + 64 * half, x2[0]);
@@ -624,17 +641,12 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) {
                         const float p0 = ex2(x[c]), p1 = ex2(x[c + 1]);
-                        if (c & 2)
-                            sum = add2(sum, pack2(p0, p1));
-                        else
-                            sum2 = add2(sum2, pack2(p0, p1));
                         p[c / 2] = pack_bf16x2(p0, p1);
+                        sum.add(c >> 1, p0, p1, p[c / 2]);
                     }
                     tmem_st16(p_t + kPHalf * half + 16 * i, p);
                 }
-                float s0, s1;
-                unpack2(add2(sum, sum2), s0, s1);
-                l += s0 + s1;
+                sum.into(l, lr);
             } else {
             float z[kRows];
 #pragma unroll
@@ -705,6 +717,7 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                 const float f = grow ? ex2(m - mb) : 1.f;
                 if (grow) m = mb;
                 l *= f;
+                lr *= f;
 #pragma unroll 1
                 for (int c = 0; c < DP; c += 32) {
                     float o[32];
@@ -718,7 +731,7 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
             const float ref = m == -INFINITY ? 0.f : m;
             const f32x2 nref = pack2(-ref, -ref), zs = pack2(g.zscale, g.zscale);
             uint32_t p[kRows / 2];
-            f32x2 sum = pack2(0.f, 0.f), sum2 = sum;
+            WeightSum sum;
 #pragma unroll
             for (int c = 0; c < kRows; c += 2) {
                 const f32x2 s2 = pack2(z[c], z[c + 1]);
@@ -726,17 +739,10 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                 unpack2(CAP || BIAS ? add2(s2, nref) : fma2(s2, zs, nref), p0, p1);
                 p0 = ex2(p0);
                 p1 = ex2(p1);
-                if (c & 2)
-                    sum = add2(sum, pack2(p0, p1));
-                else
-                    sum2 = add2(sum2, pack2(p0, p1));
                 p[c / 2] = pack_bf16x2(p0, p1);
+                sum.add(c >> 1, p0, p1, p[c / 2]);
             }
-            {
-                float s0, s1;
-                unpack2(add2(sum, sum2), s0, s1);
-                l += s0 + s1;
-            }
+            sum.into(l, lr);
             tmem_st32(p_t, p);
             tmem_st32(p_t + kPHalf, p + 32);
             }
@@ -792,12 +798,14 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
         if (ok && mbar_wait_warp(o_full + tile, 0, abort_flag, &g_attention_error)) {
             fence_after();
             if constexpr (kHalves == 2) {
-                float* s2 = sums + tile * 2 * kRows;
+                float* s2 = sums + tile * 4 * kRows;
                 s2[half * kRows + r] = l;
+                s2[(2 + half) * kRows + r] = lr;
                 meet_pair();
                 l = s2[r] + s2[kRows + r];
+                lr = s2[2 * kRows + r] + s2[3 * kRows + r];
             }
-            const float inv = hi > lo ? 1.f / l : 0.f;
+            const float inv = hi > lo ? 1.f / lr : 0.f;
             const bool live = row < g.n_q;
             uint16_t* orow = g.out + row * uint64_t(g.ldo) + uint64_t(head) * g.dim + kOCols * half;
 #pragma unroll 1
