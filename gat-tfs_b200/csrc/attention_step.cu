@@ -353,13 +353,21 @@ __global__ void __launch_bounds__(kWarps * 32) attention_step_kernel(const StepA
 }
 
 constexpr int kMostRuns = 512;  // runs are never more than this
-constexpr int kJoinGroups = 4;  // groups of 128 threads, a column each, share the pieces
+constexpr int kJoinTeams = 4;   // teams of 128 threads, a column each
 
-// Grid (segments, heads): joins the pieces of a segment that runs cut, writes
-// zeros for a segment without keys.
-__global__ void __launch_bounds__(kJoinGroups * 128) attention_join_kernel(const StepArgs a) {
-    __shared__ float f_s[kMostRuns], red[kJoinGroups * 4], acc_s[kJoinGroups][128];
-    const int seg = blockIdx.x, head = blockIdx.y, c = threadIdx.x & 127, grp = threadIdx.x >> 7;
+// Grid (segments, heads / HEADS): joins the pieces of a segment that runs cut,
+// writes zeros for a segment without keys. HEADS 1: the teams share a head's
+// pieces (few, long segments). HEADS 4: a head a team (many segments: fewer CTAs
+// that find their segment uncut).
+template <int HEADS>
+__global__ void __launch_bounds__(kJoinTeams * 128) attention_join_kernel(const StepArgs a) {
+    constexpr int kShare = kJoinTeams / HEADS;  // teams of one head
+    constexpr int kWarpsHead = 4 * kShare;
+    __shared__ float f_s[HEADS][kMostRuns], red[kJoinTeams * 4], acc_s[kJoinTeams][128];
+    const int seg = blockIdx.x, c = threadIdx.x & 127, team = threadIdx.x >> 7;
+    const int sub = HEADS == 1 ? 0 : team, share = HEADS == 1 ? team : 0;
+    const int head = blockIdx.y * HEADS + sub;
+    const bool live = head < a.heads;
     uint64_t total, start;
     count_keys(a, seg, total, start);
     const uint64_t len = seg_len(a, seg);
@@ -368,46 +376,50 @@ __global__ void __launch_bounds__(kJoinGroups * 128) attention_join_kernel(const
     const uint64_t first = len ? start / run : 0, last = len ? (start + len - 1) / run : 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the pieces are written
     if (len == 0) {
-        if (threadIdx.x < unsigned(a.dim)) out[c] = 0;
-        if (threadIdx.x == 0 && a.lse) a.lse[uint64_t(seg) * a.heads + head] = -INFINITY;
+        if (live && share == 0 && c < a.dim) out[c] = 0;
+        if (live && share == 0 && c == 0 && a.lse) a.lse[uint64_t(seg) * a.heads + head] = -INFINITY;
         return;
     }
     if (first == last) return;  // one piece: written already
     const uint64_t stride = uint64_t(a.heads) * (a.dim + 2);
-    const float* p = a.part + ((first + seg) * a.heads + head) * uint64_t(a.dim + 2);
+    const float* p = a.part + ((first + seg) * a.heads + (live ? head : 0)) * uint64_t(a.dim + 2);
     const int n = int(last - first + 1);
-    // thread i: piece i's maximum and sum
-    const bool mine = int(threadIdx.x) < n;
-    const float m = mine ? p[threadIdx.x * stride + a.dim] : -INFINITY;
-    const float l = mine ? p[threadIdx.x * stride + a.dim + 1] : 0.f;
-    float mm = warp_max(m);
+    // the pieces' maxima and sums, a thread each
+    float mm = -INFINITY;
+    for (int i = share * 128 + c; i < n; i += kShare * 128) mm = fmaxf(mm, p[i * stride + a.dim]);
+    mm = warp_max(mm);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mm;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kJoinGroups * 4; ++w) mm = fmaxf(mm, red[w]);
+    for (int w = 0; w < kWarpsHead; ++w) mm = fmaxf(mm, red[sub * kWarpsHead + w]);
     __syncthreads();
-    const float f = ex2(m - (mm == -INFINITY ? 0.f : mm));
-    if (mine) f_s[threadIdx.x] = f;
-    const float part = warp_sum(mine ? l * f : 0.f);
+    float part = 0.f;
+    for (int i = share * 128 + c; i < n; i += kShare * 128) {
+        const float f = ex2(p[i * stride + a.dim] - (mm == -INFINITY ? 0.f : mm));
+        f_s[sub][i] = f;
+        part = fmaf(p[i * stride + a.dim + 1], f, part);
+    }
+    part = warp_sum(part);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = part;
     __syncthreads();
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinGroups * 4; ++w) sum += red[w];
+    for (int w = 0; w < kWarpsHead; ++w) sum += red[sub * kWarpsHead + w];
     float acc = 0.f;
     if (c < a.dim) {
 #pragma unroll 8
-        for (int i = grp; i < n; i += kJoinGroups) acc = fmaf(p[i * stride + c], f_s[i], acc);
+        for (int i = share; i < n; i += kShare) acc = fmaf(p[i * stride + c], f_s[sub][i], acc);
     }
-    acc_s[grp][c] = acc;
-    __syncthreads();
-    if (threadIdx.x < unsigned(a.dim)) {
+    if constexpr (kShare > 1) {
+        acc_s[team][c] = acc;
+        __syncthreads();
         acc = acc_s[0][c];
 #pragma unroll
-        for (int g = 1; g < kJoinGroups; ++g) acc += acc_s[g][c];
-        out[c] = uint16_t(pack_bf16x2(acc / sum, 0.f));
+        for (int t = 1; t < kShare; ++t) acc += acc_s[t][c];
     }
-    if (threadIdx.x == 0 && a.lse) a.lse[uint64_t(seg) * a.heads + head] = (mm + log2f(sum)) * kLn2;
+    if (!live || share) return;
+    if (c < a.dim) out[c] = uint16_t(pack_bf16x2(acc / sum, 0.f));
+    if (c == 0 && a.lse) a.lse[uint64_t(seg) * a.heads + head] = (mm + log2f(sum)) * kLn2;
 }
 
 // Runs the keys are cut into: all the CTAs that fit the SMs at once (three or
@@ -488,16 +500,18 @@ int masked_attention_step_launch(const AttentionShape& s, int nseg, uint64_t n_k
     }
     GATB_LAUNCH("masked_attention_step kernel");
     if (a.runs == 1) return 0;
+    const bool many = uint64_t(nseg) * s.heads > uint64_t(2 * sms);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(nseg), unsigned(s.heads));
-    cfg.blockDim = dim3(kJoinGroups * 128);
+    cfg.gridDim = dim3(unsigned(nseg), unsigned(many ? (s.heads + 3) / 4 : s.heads));
+    cfg.blockDim = dim3(kJoinTeams * 128);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    GATB_CUDA(cudaLaunchKernelEx(&cfg, attention_join_kernel, a));
+    GATB_CUDA(many ? cudaLaunchKernelEx(&cfg, attention_join_kernel<4>, a)
+                   : cudaLaunchKernelEx(&cfg, attention_join_kernel<1>, a));
     return 0;
 }
 

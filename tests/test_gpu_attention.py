@@ -264,6 +264,12 @@ def test_step_dims_caps_and_biases(G, dev, dim, cap, bias):
     b.check(b.want(cap=cap, slopes=sl), lse=not bias)
 
 
+def test_step_many_cut_segments_odd_heads(G, dev):
+    b = Step(dev, [300, 0, 517] * 34, 6, 3, 64, seed=3)
+    b.run_step(G)
+    b.check(b.want())
+
+
 def test_step_equals_the_last_row(G, dev):
     lens = [200, 1, 77]
     b = Batch(dev, lens, lens, 4, 2, 64, seed=1)
