@@ -4,9 +4,8 @@
 // tensor core, out of tensor memory, where tcgen05.cp brings them from shared
 // memory in the tables' own tile order (fp4.cuh).
 //
-// Two kernels; fp4_product_launch chooses by the number of output tiles.
-//  pair_kernel  256 x 256 tiles of a CTA pair (cta_group::2), persistent, for
-//               outputs of at least a wave of such tiles.
+// Two kernels; launch_product chooses between them.
+//  pair_kernel  256 x 256 tiles of a CTA pair (cta_group::2), persistent.
 //  rows_kernel  128 rows of b x BN rows of a, the reduction split over a cluster
 //               and joined through distributed shared memory: few rows, small outputs.
 // Every wait is bounded (GAT_B200_ETIMEOUT through gat_b200_check_device).
@@ -294,17 +293,27 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
                         bulk_commit();
                     }
                 } else {
+                    // a lane takes 4 bytes of a row: two BF16 columns or an FP32 one
                     __syncwarp();
-                    for (int r = 0; r < 32 && row0 + r < g.m; ++r)
-                        for (int c = lane; c < width && c0 + c < g.n; c += 32) {
-                            const int byte = c * (g.out_bf16 ? 2 : 4);
-                            const uint8_t* src = sb + r * 128 + (((byte >> 4) ^ (r & 7)) * 16) + (byte & 15);
-                            const uint64_t off = (row0 + r) * uint64_t(g.ldo) + c0 + c;
-                            if (g.out_bf16)
-                                static_cast<uint16_t*>(g.out)[off] = *reinterpret_cast<const uint16_t*>(src);
-                            else
-                                static_cast<float*>(g.out)[off] = *reinterpret_cast<const float*>(src);
+                    const int live = int(min(uint64_t(32), g.m - row0));
+                    const int c = g.out_bf16 ? c0 + 2 * lane : c0 + lane;
+                    const bool pair = g.ldo % 2 == 0 && reinterpret_cast<uintptr_t>(g.out) % 4 == 0;
+                    uint8_t* o = static_cast<uint8_t*>(g.out) + (row0 * uint64_t(g.ldo) + c) * (g.out_bf16 ? 2 : 4);
+                    const uint64_t pitch = uint64_t(g.ldo) * (g.out_bf16 ? 2 : 4);
+#pragma unroll 8
+                    for (int r = 0; r < 32; ++r) {
+                        if (r >= live) break;
+                        const uint32_t w = *reinterpret_cast<const uint32_t*>(sb + r * 128 + (((lane >> 2) ^ (r & 7)) * 16) + (lane & 3) * 4);
+                        uint8_t* p = o + r * pitch;
+                        if (!g.out_bf16) {
+                            if (c < g.n) *reinterpret_cast<uint32_t*>(p) = w;
+                        } else if (pair && c + 1 < g.n) {
+                            *reinterpret_cast<uint32_t*>(p) = w;
+                        } else {
+                            if (c < g.n) *reinterpret_cast<uint16_t*>(p) = uint16_t(w);
+                            if (c + 1 < g.n) *reinterpret_cast<uint16_t*>(p + 2) = uint16_t(w >> 16);
                         }
+                    }
                     __syncwarp();
                 }
             };
@@ -345,9 +354,10 @@ constexpr int kRowsThreads = 192;
 
 template <int BN>
 struct RowsTile {
-    static constexpr int kStages = BN <= 16 ? 5 : 4;  // two CTAs an SM up to 32 rows
+    static constexpr int kStages = BN <= 16 ? 5 : BN == 64 ? 3 : 4;  // so that kCtas fit an SM's shared memory
     static constexpr int kCols = BN <= 16 ? 32 : BN;  // accumulator columns, up to 32 of scales behind them
     static constexpr int kTmem = BN <= 32 ? 64 : (BN <= 64 ? 128 : 256);
+    static constexpr int kCtas = BN <= 64 ? 2 : 1;  // an SM, by shared memory
 };
 
 template <int FORMAT, int BN>
@@ -367,7 +377,8 @@ __global__ void __launch_bounds__(kRowsThreads)
     uint64_t* full = bars;
     uint64_t* empty = full + kSt;
     uint64_t* acc_full = empty + kSt;
-    float* ra_s = reinterpret_cast<float*>(acc_full + 1);  // [BN] row scales of a
+    float* rb_s = reinterpret_cast<float*>(bars + 16);  // [128] row scales of b, [BN] of a
+    float* ra_s = rb_s + 128;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(ra_s + BN);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
     float* part = reinterpret_cast<float*>(smem);  // [BN][kPitch], over the stages once they are used up
@@ -388,9 +399,7 @@ __global__ void __launch_bounds__(kRowsThreads)
         bulk_load(f + S::kBytes, g.a_scales + ((arow >> 7) * uint64_t(g.tiles) + k * S::kTiles) * 512, 512 * sft, full + s);
     };
 
-    float rb = 1.f;
     const int q = warp & 3;
-    const int col = int(tn) * 128 + q * 32 + lane;  // output column: a row of b
     if (threadIdx.x == 0) {
         for (int s = 0; s < kSt; ++s) {
             mbar_init(full + s, 1);
@@ -407,9 +416,9 @@ __global__ void __launch_bounds__(kRowsThreads)
                      "r"(kTmem));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     } else if (warp >= 2) {
-        if (g.b_row && col < g.n) rb = g.b_row[col];
-        if (g.a_row)
-            for (int r = threadIdx.x - 64; r < BN; r += 128) ra_s[r] = arow + r < g.m ? g.a_row[arow + r] : 0.f;
+        const int i = threadIdx.x - 64, col = int(tn) * 128 + i;
+        rb_s[i] = g.b_row && col < g.n ? g.b_row[col] : 1.f;
+        for (int r = i; r < BN; r += 128) ra_s[r] = g.a_row && arow + r < g.m ? g.a_row[arow + r] : 1.f;
     }
     fence_before();
     __syncthreads();
@@ -463,15 +472,6 @@ __global__ void __launch_bounds__(kRowsThreads)
     if (warp >= 2 && ok) ok = mbar_wait(acc_full, 0, abort_flag, &g_fp4_error);
     __syncthreads();
     const int rows = int(min(uint64_t(BN), g.m - arow));
-    auto store = [&](int r, float y) {
-        if (col >= g.n) return;
-        y *= g.a_row ? rb * ra_s[r] : rb;
-        const uint64_t off = (arow + r) * uint64_t(g.ldo) + col;
-        if (g.out_bf16)
-            static_cast<uint16_t*>(g.out)[off] = uint16_t(pack_bf16x2(y, 0.f));
-        else
-            static_cast<float*>(g.out)[off] = y;
-    };
     if (warp >= 2) {
         fence_after();
 #pragma unroll 1
@@ -479,41 +479,64 @@ __global__ void __launch_bounds__(kRowsThreads)
             float v[16];
             tmem_ld16(tmem + (uint32_t(q * 32) << 16) + c, v);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float y = ok ? v[i] : 0.f;  // a CTA that gave up adds nothing
-                if (split > 1)
-                    part[(c + i) * kPitch + q * 32 + lane] = y;
-                else if (c + i < rows)
-                    store(c + i, y);
-            }
+            for (int i = 0; i < 16; ++i) part[(c + i) * kPitch + q * 32 + lane] = ok ? v[i] : 0.f;
         }
         fence_before();
     }
-    if (split > 1) {
+    if (split > 1)
         cluster_sync();
-        if (warp >= 2) {
-            // rows rank, rank + split, ...: four rows' loads from the cluster in flight at a time
-            for (int r0 = int(rank); r0 < rows; r0 += 4 * split) {
-                float y[4] = {0.f, 0.f, 0.f, 0.f};
-                for (int c = 0; c < split; ++c) {
-                    const uint32_t base = map_to_rank(smem_u32(part), uint32_t(c));
+    else
+        __syncthreads();
+    if (warp >= 2) {
+        // rows rank, rank + split, ..: a thread takes four columns of a row from every CTA of the cluster
+        const int mine = (rows - int(rank) + split - 1) / split;
+        const int es = g.out_bf16 ? 2 : 4;
+        const bool vec = g.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(g.out) % (4 * es) == 0;
+#pragma unroll 2
+        for (int it = threadIdx.x - 64; it < mine * 32; it += 128) {
+            const int r = int(rank) + (it >> 5) * split, c = (it & 31) * 4, col = int(tn) * 128 + c;
+            float y[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint32_t at = smem_u32(part + r * kPitch + c);
+            for (int i = 0; i < split; ++i) {
+                float x[4];
+                asm("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                    : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
+                    : "r"(split > 1 ? map_to_rank(at, uint32_t(i)) : at)
+                    : "memory");
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = min(r0 + i * split, BN - 1);
-                        float x;
-                        asm("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(base + (r * kPitch + q * 32 + lane) * 4) : "memory");
-                        y[i] += x;
-                    }
+                for (int e = 0; e < 4; ++e) y[e] += x[e];
+            }
+            const float ra = ra_s[r];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] *= ra * rb_s[c + e];
+            const uint64_t off = (arow + r) * uint64_t(g.ldo) + col;
+            if (g.out_bf16) {
+                uint16_t* o = static_cast<uint16_t*>(g.out) + off;
+                const uint32_t lo = pack_bf16x2(y[0], y[1]), hi = pack_bf16x2(y[2], y[3]);
+                if (vec && col + 4 <= g.n) {
+                    *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
+                } else {
+                    if (col < g.n) o[0] = uint16_t(lo);
+                    if (col + 1 < g.n) o[1] = uint16_t(lo >> 16);
+                    if (col + 2 < g.n) o[2] = uint16_t(hi);
+                    if (col + 3 < g.n) o[3] = uint16_t(hi >> 16);
                 }
+            } else {
+                float* o = static_cast<float*>(g.out) + off;
+                if (vec && col + 4 <= g.n) {
+                    *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
+                } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (r0 + i * split < rows) store(r0 + i * split, y[i]);
+                    for (int e = 0; e < 4; ++e)
+                        if (col + e < g.n) o[e] = y[e];
+                }
             }
         }
-        cluster_sync();  // the others have read this CTA's part
-    } else {
-        __syncthreads();
     }
+    if (split > 1)
+        cluster_sync();  // the others have read this CTA's part
+    else
+        __syncthreads();
     if (warp == 1) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmem));
@@ -569,22 +592,28 @@ int launch_pair(ProductArgs g, const void* a, int lda, const void* b, int ldb, i
     return 0;
 }
 
+// Parts that the rows kernel splits the reduction into: while all of them run at
+// once and each keeps two stages.
+int rows_split(uint64_t tiles, int stages_k, uint64_t slots) {
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= slots && stages_k >= 4 * split) split *= 2;
+    return split;
+}
+
 template <int FORMAT, int BN>
 int launch_rows(ProductArgs g, const void* a, int lda, const void* b, int ldb, int kb, int sms, cudaStream_t st) {
     using S = Scales<FORMAT>;
     g.grid_m = uint32_t((g.m + BN - 1) / BN);
     g.grid_n = uint32_t((g.n + 127) / 128);
     const uint64_t tiles = uint64_t(g.grid_m) * g.grid_n;
-    // split the reduction while that leaves CTAs for idle SMs and each part two stages
-    int split = 1;
-    while (split < 8 && tiles * split < uint64_t(sms) && g.stages_k >= 4 * split) split *= 2;
+    const int split = rows_split(tiles, g.stages_k, uint64_t(sms) * RowsTile<BN>::kCtas);
     CUtensorMap tm_a, tm_b;
     if (int rc = codes_map(&tm_a, a, g.m, kb, lda, BN)) return rc;
     if (int rc = codes_map(&tm_b, b, uint64_t(g.n), kb, ldb, 128)) return rc;
     constexpr int stages = RowsTile<BN>::kStages * (128 * 128 + BN * 128 + 2 * S::kBytes);
     constexpr int part = BN * 132 * 4;
     static_assert(part <= stages, "the exchange buffer lies over the stages");
-    constexpr int smem = stages + 256 + BN * 4 + 1024;
+    constexpr int smem = stages + 256 + (128 + BN) * 4 + 1024;
     auto kern = rows_kernel<FORMAT, BN>;
     GATB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg{};
@@ -605,12 +634,22 @@ int launch_rows(ProductArgs g, const void* a, int lda, const void* b, int ldb, i
 template <int FORMAT>
 int launch_product(const ProductArgs& g, const void* a, int lda, const void* b, int ldb, int kb, int sms,
                    cudaStream_t st) {
-    const uint64_t pair_tiles = (g.m + 255) / 256 * ((uint64_t(g.n) + 255) / 256);
-    if (pair_tiles >= uint64_t(sms / 2)) return launch_pair<FORMAT>(g, a, lda, b, ldb, kb, sms, st);
+    // Up to 64 rows the rows kernel (64 x 8192 x 2048: both 8.4 us; 33 x 8192 x 8192: 10 us, pairs 16;
+    // 48 x 20000 x 1024: 8.6 us, pairs 9.6). Above, whichever these times, fitted to both, give the lead:
+    // a pair kernel takes 5.3 us and 0.35 us a stage and wave, a rows kernel 9 us and as much a stage of
+    // its part (100 x 1000 x 8192: 9.6 us, pairs 16.3; 100 x 4096 x 1024: 9.3 us, pairs 7.5;
+    // 2000 x 2000 x 8192: 47 us, pairs 18.6).
     if (g.m <= 16) return launch_rows<FORMAT, 16>(g, a, lda, b, ldb, kb, sms, st);
     if (g.m <= 32) return launch_rows<FORMAT, 32>(g, a, lda, b, ldb, kb, sms, st);
     if (g.m <= 64) return launch_rows<FORMAT, 64>(g, a, lda, b, ldb, kb, sms, st);
-    return launch_rows<FORMAT, 128>(g, a, lda, b, ldb, kb, sms, st);
+    const uint64_t pair_tiles = (g.m + 255) / 256 * ((uint64_t(g.n) + 255) / 256), pairs = uint64_t(sms) / 2;
+    const uint64_t tiles = (g.m + 127) / 128 * ((uint64_t(g.n) + 127) / 128);
+    const int split = rows_split(tiles, g.stages_k, uint64_t(sms));
+    const double by_pairs = 5.3 + 0.35 * g.stages_k * double((pair_tiles + pairs - 1) / pairs);
+    const double by_rows = (split == 1 ? 11.0 : 9.0) +
+                           0.35 * ((g.stages_k + split - 1) / split) * double((tiles * split + sms - 1) / sms);
+    return by_pairs <= by_rows ? launch_pair<FORMAT>(g, a, lda, b, ldb, kb, sms, st)
+                               : launch_rows<FORMAT, 128>(g, a, lda, b, ldb, kb, sms, st);
 }
 
 }  // namespace
