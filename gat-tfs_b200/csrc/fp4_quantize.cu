@@ -48,77 +48,142 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
     return r;
 }
 
-// 8 columns from element offset `off`, of which `valid` exist (zeros behind).
-// VEC: fours of columns are whole and aligned.
-template <bool BF16, bool VEC>
-__device__ __forceinline__ void load8(const void* x, uint64_t off, int valid, float* v) {
-    if constexpr (BF16) {
-        const uint16_t* p = static_cast<const uint16_t*>(x) + off;
-        uint32_t u[4] = {0u, 0u, 0u, 0u};
-        if constexpr (VEC) {
-            if (valid > 0) {
-                const uint2 t = __ldg(reinterpret_cast<const uint2*>(p));
-                u[0] = t.x;
-                u[1] = t.y;
-            }
-            if (valid > 4) {
-                const uint2 t = __ldg(reinterpret_cast<const uint2*>(p) + 1);
-                u[2] = t.x;
-                u[3] = t.y;
-            }
+// Memory is touched in fours: 4 elements at an address that is a multiple of
+// their size. LOOSE: rows may begin and end inside a four, and a lane's 8
+// columns then lie in up to three of them. A four with elements outside the
+// row is taken apart. 58,798 x 3782 BF16 to NVFP4 took 540 us element by
+// element and takes 275, 100,000 x 501 FP32 to MXFP4 133 and 78.
+
+// The four at p, whose first element is column `col` of the row.
+template <bool BF16, bool LOOSE>
+__device__ __forceinline__ void load4(const void* p, int col, int width, uint32_t* u) {
+    constexpr int kWords = BF16 ? 2 : 4;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) u[i] = 0u;
+    if (LOOSE ? col >= 0 && col + 4 <= width : col < width) {
+        if constexpr (BF16) {
+            const uint2 t = __ldg(static_cast<const uint2*>(p));
+            u[0] = t.x; u[1] = t.y;
         } else {
+            const uint4 t = __ldg(static_cast<const uint4*>(p));
+            u[0] = t.x; u[1] = t.y; u[2] = t.z; u[3] = t.w;
+        }
+    } else if (LOOSE && col > -4 && col < width) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t lo = 2 * i < valid ? __ldg(p + 2 * i) : 0u;
-                const uint32_t hi = 2 * i + 1 < valid ? __ldg(p + 2 * i + 1) : 0u;
-                u[i] = lo | (hi << 16);
+        for (int i = 0; i < 4; ++i)
+            if (col + i >= 0 && col + i < width) {
+                if constexpr (BF16)
+                    u[i / 2] |= uint32_t(__ldg(static_cast<const uint16_t*>(p) + i)) << (i % 2 * 16);
+                else
+                    u[i] = __ldg(static_cast<const uint32_t*>(p) + i);
             }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = bf16lo(u[i]);
-            v[2 * i + 1] = bf16hi(u[i]);
-        }
-    } else {
-        const float* p = static_cast<const float*>(x) + off;
-        if constexpr (VEC) {
-            float4 t0 = make_float4(0.f, 0.f, 0.f, 0.f), t1 = t0;
-            if (valid > 0) t0 = __ldg(reinterpret_cast<const float4*>(p));
-            if (valid > 4) t1 = __ldg(reinterpret_cast<const float4*>(p) + 1);
-            v[0] = t0.x; v[1] = t0.y; v[2] = t0.z; v[3] = t0.w;
-            v[4] = t1.x; v[5] = t1.y; v[6] = t1.z; v[7] = t1.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = i < valid ? __ldg(p + i) : 0.f;
-        }
     }
 }
-// The same for the values: y to element offset `off`.
-template <bool VEC>
-__device__ __forceinline__ void store8(void* out, bool bf16, uint64_t off, int valid, const float* y) {
-    if (bf16) {  // the values have at most six significant bits
-        uint16_t* p = static_cast<uint16_t*>(out) + off;
-        uint32_t w[4];
+// Its columns from `first` to the width.
+template <bool BF16, bool LOOSE>
+__device__ __forceinline__ void store4(void* p, int col, int first, int width, const uint32_t* u) {
+    if (LOOSE ? col >= first && col + 4 <= width : col < width) {
+        if constexpr (BF16)
+            *static_cast<uint2*>(p) = make_uint2(u[0], u[1]);
+        else
+            *static_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+    } else if (LOOSE && col > first - 4 && col < width) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(y[2 * i], y[2 * i + 1]);
-        if constexpr (VEC) {
-            if (valid > 0) reinterpret_cast<uint2*>(p)[0] = make_uint2(w[0], w[1]);
-            if (valid > 4) reinterpret_cast<uint2*>(p)[1] = make_uint2(w[2], w[3]);
+        for (int i = 0; i < 4; ++i)
+            if (col + i >= first && col + i < width) {
+                if constexpr (BF16)
+                    static_cast<uint16_t*>(p)[i] = uint16_t(u[i / 2] >> (i % 2 * 16));
+                else
+                    static_cast<uint32_t*>(p)[i] = u[i];
+            }
+    }
+}
+
+// Columns [col, col + 8) of the row at element offset `off`; zeros past the width.
+template <bool BF16, bool LOOSE>
+__device__ __forceinline__ void load8(const void* x, uint64_t off, int col, int width, float* v) {
+    constexpr int kWords = BF16 ? 2 : 4, kSize = BF16 ? 2 : 4;  // words of a four, bytes of an element
+    const char* p = static_cast<const char*>(x) + (off + uint64_t(col)) * kSize;
+    uint32_t u[3 * kWords];
+    if constexpr (LOOSE) {
+        const int s = int(reinterpret_cast<uintptr_t>(p) / kSize & 3);
+        p -= s * kSize;
+        load4<BF16, true>(p, col - s, width, u);
+        load4<BF16, true>(p + 4 * kSize, col - s + 4, width, u + kWords);
+        load4<BF16, true>(p + 8 * kSize, col - s + 8, s ? width : 0, u + 2 * kWords);
+        if constexpr (BF16) {
+#pragma unroll
+            for (int i = 0; i < 5; ++i) u[i] = s & 2 ? u[i + 1] : u[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = __funnelshift_r(u[i], u[i + 1], s & 1 ? 16 : 0);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < valid) p[i] = uint16_t(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
+            for (int i = 0; i < 9; ++i) u[i] = s & 2 ? u[i + 2] : u[i];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = s & 1 ? u[i + 1] : u[i];
         }
     } else {
-        float* p = static_cast<float*>(out) + off;
-        if constexpr (VEC) {
-            if (valid > 0) reinterpret_cast<float4*>(p)[0] = make_float4(y[0], y[1], y[2], y[3]);
-            if (valid > 4) reinterpret_cast<float4*>(p)[1] = make_float4(y[4], y[5], y[6], y[7]);
+        load4<BF16, false>(p, col, width, u);
+        load4<BF16, false>(p + 4 * kSize, col + 4, width, u + kWords);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (BF16)
+            v[i] = i % 2 ? bf16hi(u[i / 2]) : bf16lo(u[i / 2]);
+        else
+            v[i] = __uint_as_float(u[i]);
+    }
+}
+
+// y to columns [col, col + 8) of the row at element offset `off`, up to the
+// width. LOOSE: the whole warp calls it, `group` neighbouring lanes with
+// neighbouring columns of a row. A lane stores the two fours that end in its
+// columns, with up to three elements of the lane before it in the first; the
+// group's last lane stores the elements behind them too.
+template <bool BF16, bool LOOSE>
+__device__ __forceinline__ void store8(void* out, uint64_t off, int col, int width, const float* y, int group) {
+    constexpr int kWords = BF16 ? 2 : 4, kSize = BF16 ? 2 : 4;
+    char* p = static_cast<char*>(out) + (off + uint64_t(col)) * kSize;
+    uint32_t u[3 * kWords];  // columns [col - 4, col + 8)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (!BF16)
+            u[kWords + i] = __float_as_uint(y[i]);
+        else if (i % 2 == 0)
+            u[kWords + i / 2] = pack_bf16x2(y[i], y[i + 1]);  // exact: at most six significant bits
+    }
+    if constexpr (LOOSE) {
+        const int s = int(reinterpret_cast<uintptr_t>(p) / kSize & 3), at = threadIdx.x % group;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) u[i] = __shfl_up_sync(0xffffffffu, u[2 * kWords + i], 1);
+        if (at == group - 1) {
+#pragma unroll
+            for (int i = 5; i < 8; ++i)
+                if (i >= 8 - s && col + i < width) {
+                    if constexpr (BF16)
+                        reinterpret_cast<uint16_t*>(p)[i] = uint16_t(u[kWords + i / 2] >> (i % 2 * 16));
+                    else
+                        reinterpret_cast<uint32_t*>(p)[i] = u[kWords + i];
+                }
+        }
+        if constexpr (BF16) {  // to columns [col - s, col - s + 8) from the second four on
+#pragma unroll
+            for (int i = 5; i >= 1; --i) u[i] = s & 2 ? u[i - 1] : u[i];
+#pragma unroll
+            for (int i = 5; i >= 2; --i) u[i] = __funnelshift_l(u[i - 1], u[i], s & 1 ? 16 : 0);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < valid) p[i] = y[i];
+            for (int i = 11; i >= 3; --i) u[i] = s & 2 ? u[i - 2] : u[i];
+#pragma unroll
+            for (int i = 11; i >= 4; --i) u[i] = s & 1 ? u[i - 1] : u[i];
         }
+        p -= s * kSize;
+        const int first = at == 0 ? col : 0;
+        store4<BF16, true>(p, col - s, first, width, u + kWords);
+        store4<BF16, true>(p + 4 * kSize, col - s + 4, first, width, u + 2 * kWords);
+    } else {
+        store4<BF16, false>(p, col, 0, width, u + kWords);
+        store4<BF16, false>(p + 4 * kSize, col + 4, 0, width, u + 2 * kWords);
     }
 }
 
@@ -184,15 +249,15 @@ __device__ __forceinline__ float reciprocal_e4m3(float s) {
     return fmaf(y, fmaf(-s, y, 1.f), y);
 }
 
-// LANES lanes per row (16 or 32: part of a warp; 256: the CTA), CHUNKS pieces
+// LANES lanes per row (4 to 32: part of a warp; 256: the CTA), CHUNKS pieces
 // of 8 columns a lane kept in registers. REREAD: rows longer than LANES *
-// CHUNKS * 8 columns are read a second time for the codes. VEC: width, rows of
-// x and rows of the values are whole, aligned fours of elements.
+// CHUNKS * 8 columns are read a second time for the codes. LOOSE: width, rows of
+// x or rows of the values are not all whole, aligned fours of elements.
 // Issue slots bind it as much as memory does, hence packed FP32 pairs and no
 // branches on alignment inside: 2,449,029 x 100 FP32 to NVFP4 with BF16 values
 // took 389 us with scalar arithmetic and such branches and takes 294 us
 // (5.5 TB/s); 169,343 x 128 FP32 to MXFP4 25 us (5.6 TB/s).
-template <int FORMAT, bool BF16, bool VEC, int LANES, int CHUNKS, bool REREAD>
+template <int FORMAT, bool BF16, bool LOOSE, int LANES, int CHUNKS, bool REREAD>
 __global__ void __launch_bounds__(256) fp4_quantize_kernel(const QuantArgs a) {
     constexpr bool kNv = FORMAT == GAT_B200_NVFP4;
     constexpr int kBlockLanes = fp4_block(FORMAT) / 8;  // lanes of one block
@@ -208,7 +273,12 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(const QuantArgs a) {
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
             const int col = ((c0 + c) * LANES + lane) * 8;
-            load8<BF16, VEC>(a.x, xoff + uint64_t(col), width - col, v[c]);
+            if (LOOSE && (c0 + c) * LANES * 8 >= a.width) {  // the same for all lanes
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[c][i] = 0.f;
+            } else {
+                load8<BF16, LOOSE>(a.x, xoff, col, width, v[c]);
+            }
         }
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
@@ -284,19 +354,25 @@ __global__ void __launch_bounds__(256) fp4_quantize_kernel(const QuantArgs a) {
                 unpack2(q2, q[i], q[i + 1]);
             }
             const uint32_t code = inv == 0.f ? 0u : e2m1x8(q);
-            if (!live || chunk >= a.chunks) continue;
-            if (chunk < a.code_chunks) *reinterpret_cast<uint32_t*>(code_row + uint32_t(chunk) * 4) = code;
-            if (lane % kBlockLanes == 0) {
-                const uint32_t block = uint32_t(chunk) / kBlockLanes;
-                scale_row[uint64_t(block >> 2) * 512 + (block & 3)] = uint8_t(byte);
+            if (live && chunk < a.chunks) {
+                if (chunk < a.code_chunks) *reinterpret_cast<uint32_t*>(code_row + uint32_t(chunk) * 4) = code;
+                if (lane % kBlockLanes == 0) {
+                    const uint32_t block = uint32_t(chunk) / kBlockLanes;
+                    scale_row[uint64_t(block >> 2) * 512 + (block & 3)] = uint8_t(byte);
+                }
             }
-            if (a.values) {
+            if (a.values && (!LOOSE || (s * CHUNKS + c) * LANES * 8 < a.width)) {
                 float y[8];
                 from_e2m1x8(code, y);
                 const f32x2 d2 = pack2(d, d);
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) unpack2(mul2(pack2(y[i], y[i + 1]), d2), y[i], y[i + 1]);
-                store8<VEC>(a.values, a.v_bf16, row * uint64_t(a.ldv) + uint64_t(chunk) * 8, width - chunk * 8, y);
+                constexpr int kGroup = LANES < 32 ? LANES : 32;
+                const uint64_t off = row * uint64_t(a.ldv);
+                if (a.v_bf16)
+                    store8<true, LOOSE>(a.values, off, chunk * 8, width, y, kGroup);
+                else
+                    store8<false, LOOSE>(a.values, off, chunk * 8, width, y, kGroup);
             }
         }
     }
@@ -308,34 +384,42 @@ int row_align(const void* base, uint64_t pitch) {
     return int(u & (~u + 1));
 }
 
-template <int FORMAT, bool BF16, bool VEC>
+template <int FORMAT, bool BF16, bool LOOSE>
 int launch_quantize(const QuantArgs& a, cudaStream_t st) {
-    // 16 or 32 lanes a row while a row fits them once, one warp up to 1024
+    // As many lanes a row as its pieces take, up to a warp; one warp up to 1024
     // columns, the CTA for longer ones; above 8192 columns NVFP4 reads twice.
+    // Up to 32 columns 4 lanes, as most of a scale tile is empty (305,316 x 32
+    // FP32 to MXFP4: 25 us, 16 lanes 35; to NVFP4 18 us, 16 lanes 22).
+    constexpr int kFew = FORMAT == GAT_B200_MXFP4 ? 4 : 2;  // pieces a lane of a scale tile
+    const unsigned per64 = unsigned((a.n + 63) / 64), per32 = unsigned((a.n + 31) / 32);
     const unsigned per16 = unsigned((a.n + 15) / 16), per8 = unsigned((a.n + 7) / 8), n = unsigned(a.n);
-    if (a.chunks <= 16)
-        fp4_quantize_kernel<FORMAT, BF16, VEC, 16, 1, false><<<per16, 256, 0, st>>>(a);
+    if (a.width <= 32)
+        fp4_quantize_kernel<FORMAT, BF16, LOOSE, 4, kFew, false><<<per64, 256, 0, st>>>(a);
+    else if (FORMAT == GAT_B200_NVFP4 && a.chunks <= 8)
+        fp4_quantize_kernel<GAT_B200_NVFP4, BF16, LOOSE, 8, 1, false><<<per32, 256, 0, st>>>(a);
+    else if (a.chunks <= 16)
+        fp4_quantize_kernel<FORMAT, BF16, LOOSE, 16, 1, false><<<per16, 256, 0, st>>>(a);
     else if (a.chunks <= 32)
-        fp4_quantize_kernel<FORMAT, BF16, VEC, 32, 1, false><<<per8, 256, 0, st>>>(a);
+        fp4_quantize_kernel<FORMAT, BF16, LOOSE, 32, 1, false><<<per8, 256, 0, st>>>(a);
     else if (a.chunks <= 64)
-        fp4_quantize_kernel<FORMAT, BF16, VEC, 32, 2, false><<<per8, 256, 0, st>>>(a);
+        fp4_quantize_kernel<FORMAT, BF16, LOOSE, 32, 2, false><<<per8, 256, 0, st>>>(a);
     else if (a.chunks <= 128)
-        fp4_quantize_kernel<FORMAT, BF16, VEC, 32, 4, false><<<per8, 256, 0, st>>>(a);
+        fp4_quantize_kernel<FORMAT, BF16, LOOSE, 32, 4, false><<<per8, 256, 0, st>>>(a);
     else if (a.chunks <= 256)
-        fp4_quantize_kernel<FORMAT, BF16, VEC, 256, 1, false><<<n, 256, 0, st>>>(a);
+        fp4_quantize_kernel<FORMAT, BF16, LOOSE, 256, 1, false><<<n, 256, 0, st>>>(a);
     else if (a.chunks <= 512)
-        fp4_quantize_kernel<FORMAT, BF16, VEC, 256, 2, false><<<n, 256, 0, st>>>(a);
+        fp4_quantize_kernel<FORMAT, BF16, LOOSE, 256, 2, false><<<n, 256, 0, st>>>(a);
     else if (a.chunks <= 1024)
-        fp4_quantize_kernel<FORMAT, BF16, VEC, 256, 4, false><<<n, 256, 0, st>>>(a);
+        fp4_quantize_kernel<FORMAT, BF16, LOOSE, 256, 4, false><<<n, 256, 0, st>>>(a);
     else
-        fp4_quantize_kernel<FORMAT, BF16, VEC, 256, 4, true><<<n, 256, 0, st>>>(a);
+        fp4_quantize_kernel<FORMAT, BF16, LOOSE, 256, 4, true><<<n, 256, 0, st>>>(a);
     GATB_LAUNCH("fp4_quantize kernel");
     return 0;
 }
 template <int FORMAT>
-int launch_quantize(const QuantArgs& a, bool bf16, bool vec, cudaStream_t st) {
-    if (bf16) return vec ? launch_quantize<FORMAT, true, true>(a, st) : launch_quantize<FORMAT, true, false>(a, st);
-    return vec ? launch_quantize<FORMAT, false, true>(a, st) : launch_quantize<FORMAT, false, false>(a, st);
+int launch_quantize(const QuantArgs& a, bool bf16, bool loose, cudaStream_t st) {
+    if (bf16) return loose ? launch_quantize<FORMAT, true, true>(a, st) : launch_quantize<FORMAT, true, false>(a, st);
+    return loose ? launch_quantize<FORMAT, false, true>(a, st) : launch_quantize<FORMAT, false, false>(a, st);
 }
 
 }  // namespace
@@ -380,11 +464,11 @@ int fp4_quantize_launch(int format, uint64_t n, int width, const void* x, int x_
     a.values = values;
     a.ldv = ldv;
     a.v_bf16 = v_dtype == GAT_B200_BF16;
-    const bool vec = width % 4 == 0 && row_align(x, uint64_t(ldx) * xs) >= 4 * xs &&
-                     (!values || row_align(values, uint64_t(ldv) * vs) >= 4 * vs);
+    const bool loose = !(width % 4 == 0 && row_align(x, uint64_t(ldx) * xs) >= 4 * xs &&
+                         (!values || row_align(values, uint64_t(ldv) * vs) >= 4 * vs));
     const bool bf16 = x_dtype == GAT_B200_BF16;
-    return format == GAT_B200_MXFP4 ? launch_quantize<GAT_B200_MXFP4>(a, bf16, vec, st)
-                                    : launch_quantize<GAT_B200_NVFP4>(a, bf16, vec, st);
+    return format == GAT_B200_MXFP4 ? launch_quantize<GAT_B200_MXFP4>(a, bf16, loose, st)
+                                    : launch_quantize<GAT_B200_NVFP4>(a, bf16, loose, st);
 }
 
 }  // namespace gatb

@@ -116,6 +116,18 @@ def test_quantize_strides_and_alignment(G, dev, fmt, dtype, pad, offset, v32):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("offset,pad,vpad,v32", [(1, 0, 3, False), (3, 2, 1, True), (0, 5, 2, False), (2, 3, 0, True)])
+@pytest.mark.parametrize("n,w", [(150, 1), (70, 2), (67, 30), (40, 63), (35, 126), (19, 129), (9, 255), (6, 509),
+                                 (5, 1023), (3, 2045), (3, 4001), (2, 8190), (2, 8203)])
+def test_quantize_rows_that_begin_and_end_anywhere(G, dev, fmt, dtype, n, w, offset, pad, vpad, v32):
+    x = features(n, w, 31 * n + w, dtype)
+    got = quantize(G, x, fmt, dtype, dev, ldx=w + pad, extra_ldc=0, v_dtype=G.F32 if v32 else G.BF16, extra_ldv=vpad,
+                   offset=offset)
+    check(G, got, x, fmt)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_quantize_borders_and_ties(G, dev, fmt):
     # every rounding border of E2M1 at every block scale, with its neighbours in FP32
     borders = np.array([.25, .75, 1.25, 1.75, 2.5, 3.5, 5.0], np.float32)
