@@ -63,7 +63,7 @@ struct AttnArgs {
     int ldv;
     float zscale;    // without a cap: scale * log2 e; with one: scale / cap
     float zcap;      // cap * log2 e
-    float small;     // raw scores up to which the tanh's long polynomial holds (half of it: the short one)
+    float small;     // raw scores up to which the tanh's long polynomial holds (a third of it: the short one)
     float tanh[5];   // coefficients of s, s^3 .. in zcap tanh(scale / cap * s)
     float tanh3[3];
     uint16_t* out;
@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                     top2 = max3(top2, fabsf(x2[1][c]), fabsf(x2[1][c + 1]));
                 }
                 top = fmaxf(top, top2);
-                const int degree = __all_sync(0xffffffffu, top <= 0.5f * g.small) ? 3
+                const int degree = __all_sync(0xffffffffu, top <= g.small * (1.f / 3.f)) ? 3
                                    : __all_sync(0xffffffffu, top <= g.small)      ? 5
                                                                                   : 0;
 #pragma unroll

@@ -24,11 +24,11 @@ __device__ __forceinline__ float rcp(float x) {
 __device__ __forceinline__ float tanh_of_log2(float x) { return fmaf(-2.f, rcp(ex2(x) + 1.f), 1.f); }
 
 // tanh(x) = x p(x^2), minimax polynomials (Remez exchange): five terms for
-// |x| <= 0.6, relative error 7.4e-8, and three for |x| <= 0.3, 1.2e-6 (of a
-// score of at most 0.3 cap).
+// |x| <= 0.6, relative error 7.4e-8, and three for |x| <= 0.2, 1.2e-7 (for
+// |x| <= 0.3 it would be 1.2e-6, and show in the log-sum-exp).
 constexpr float kTanhLimit = 0.6f;
 constexpr float kTanh[5] = {0.999999926872f, -0.333323099889f, 0.133101737673f, -0.0521014822761f, 0.0154754278422f};
-constexpr float kTanhShort[3] = {0.99999883885f, -0.33310021606f, 0.126339459906f};
+constexpr float kTanhShort[3] = {0.9999999f, -0.3332859f, 0.13015407f};
 // cap log2 e tanh(t), t = scale s / cap, for any cap and score: where tanh(t)
 // is small against 1 the exponentials would cancel.
 __device__ __forceinline__ float capped_score(float t, float zcap) {
