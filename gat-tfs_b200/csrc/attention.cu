@@ -23,8 +23,9 @@
 // The running maximum is only moved when it grows by more than 24 (weights up
 // to 2^24, far inside FP32 and BF16's range), so O is seldom rescaled.
 // MMAs of a CTA run in order, so where P overlays S, S's barrier also says that
-// the tile's last P V is done and O is at rest. P is rounded to BF16 (the tensor cores' input type;
-// the sum keeps the unrounded FP32 weights).
+// the tile's last P V is done and O is at rest. P is rounded to BF16 (the tensor cores' input
+// type); out is divided by the FP32 sum of the rounded weights, so a row is an
+// average with its own weights, and lse takes the sum of the unrounded ones.
 // The exponentials bound it (16 a clock and SM; a 128 x 128 block of dim 128
 // takes the tensor cores as long as its exponentials): the cap's tanh is a
 // polynomial on the FMA pipe wherever a block's scores stay below 0.6 cap. A

@@ -423,12 +423,13 @@ __global__ void __launch_bounds__(kJoinTeams * 128) attention_join_kernel(const 
 }
 
 // Runs the keys are cut into: all the CTAs that fit the SMs at once (three or
-// two an SM by their registers), no more than there can be pieces for (119
-// segments of up to 9 keys took 55 us in runs counted by their keys alone).
+// two an SM by their registers), no more than there can be pieces for, also
+// where segments share keys (119 segments of up to 9 keys took 55 us in as many
+// runs as their keys fill, and take 9).
 int step_runs(int kv_heads, int group, int dim, uint64_t n_k, int nseg, int sms) {
     const int columns = kv_heads * ((group + kHeadTile - 1) / kHeadTile);
     const uint64_t want = uint64_t((dim <= 64 ? 3 : 2) * sms / columns);
-    const uint64_t most = (n_k + kWarps * kKeys - 1) / (kWarps * kKeys) + uint64_t(nseg) - 1;
+    const uint64_t most = (n_k + kWarps * kKeys - 1) / (kWarps * kKeys) * uint64_t(nseg);
     const uint64_t runs = want < most ? want : most;
     return runs < 1 ? 1 : runs > uint64_t(kMostRuns) ? kMostRuns : int(runs);
 }

@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(kRowsThreads)
             const uint32_t at = smem_u32(part + r * kPitch + c);
             for (int i = 0; i < split; ++i) {
                 float x[4];
-                asm("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
                     : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
                     : "r"(split > 1 ? map_to_rank(at, uint32_t(i)) : at)
                     : "memory");

@@ -263,7 +263,7 @@ uint64_t gat_b200_fp4_scale_bytes(int format, uint64_t n, int width);
  * or NaN gets a NaN scale: all of it reads as NaN. If values is not NULL, what
  * the table stands for is written there (FP32 or BF16, [n][ldv]; exact in
  * both, but for magnitudes below the type's normal range). Scale bytes of rows
- * past n are left as they were. */
+ * past n are left as they were. x and what is written do not overlap. */
 int gat_b200_fp4_quantize(int format, uint64_t n, int width, const void* x, int x_dtype, int ldx,
                           void* codes, int ldc, void* scales, float* row_scale, void* values,
                           int v_dtype, int ldv, void* stream);

@@ -294,6 +294,15 @@ def test_step_overlapping_and_cut_segments(G, dev):
     b.check(want)
 
 
+def test_step_many_segments_over_the_same_keys(G, dev):
+    b = Step(dev, [700], 4, 1, 64, seed=8)
+    b.q = torch.randn(43, 256, device=dev).to(torch.bfloat16)
+    b.out, b.lse = b.out[:1].repeat(43, 1), b.lse[:1].repeat(43, 1)
+    b.nq, b.lens, b.begin = 40, [700 - 3 * i for i in range(40)], [i for i in range(40)]
+    b.run_step(G, 20.0)
+    b.check(b.want(cap=20.0))
+
+
 def test_step_non_finite_neighbours(G, dev):
     lens = [40, 60, 129]
     a, b = Step(dev, lens, 4, 2, 64, seed=7, gap=3), Step(dev, lens, 4, 2, 64, seed=7, gap=3)
