@@ -119,60 +119,56 @@ __global__ void __launch_bounds__(kWarps * 32) attention_step_kernel(const StepA
             if (a.lse && int(threadIdx.x) < live_heads) a.lse[uint64_t(s) * a.heads + head0 + threadIdx.x] = -INFINITY;
         }
     }
-    // Where this run lies. Up to one segment a thread, one pass over them gives
-    // the total, the first segment and, in shared memory, every segment's keys.
-    constexpr int kThreads = kWarps * 32;
-    __shared__ uint64_t sums[kWarps], len_s[kThreads], begin_s[kThreads];
+    // Where this run lies: a thread adds up the places of neighbouring segments, a
+    // scan over the threads gives the total and the first segment of the run. Up
+    // to kKept segments' keys stay in shared memory (300 segments of 40 keys,
+    // 16/4 x 128: 29 us with two passes and reads in between, now 27).
+    constexpr int kThreads = kWarps * 32, kKept = 512;
+    __shared__ uint64_t sums[kWarps], len_s[kKept], begin_s[kKept];
     __shared__ int found;
     __shared__ uint64_t found_start;
-    const bool few = a.nseg <= kThreads;
-    uint64_t total, unused;
-    if (!few) count_keys(a, 0, total, unused);
-    if (threadIdx.x == 0) found = -1;
-    int seg = 0;
-    uint64_t seg_start = 0;  // places before it
-    uint64_t run = few ? 0 : run_places(total, a.runs);
-    uint64_t v0 = run * blockIdx.x, v1 = few ? 0 : min(total, v0 + run);
-    if (!few && v0 >= v1) return;
-    for (int base = 0; base < a.nseg; base += kThreads) {
-        const int s = base + threadIdx.x;
-        const uint64_t len = s < a.nseg ? seg_len(a, s) : 0, l = seg_places(len);
-        if (few) {
-            len_s[threadIdx.x] = len;
-            begin_s[threadIdx.x] = s < a.nseg ? a.begin[s] : 0;
+    const bool kept = a.nseg <= kKept;
+    const int each = (a.nseg + kThreads - 1) / kThreads;
+    const int s0 = min(a.nseg, int(threadIdx.x) * each), s1 = min(a.nseg, s0 + each);
+    uint64_t places = 0;
+    for (int s = s0; s < s1; ++s) {
+        const uint64_t len = seg_len(a, s);
+        if (kept) {
+            len_s[s] = len;
+            begin_s[s] = a.begin[s];
         }
-        uint64_t inc = l;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += y;
-        }
-        if (lane == 31) sums[warp] = inc;
-        __syncthreads();
-        uint64_t off = seg_start, all = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) off += sums[w];
-            all += sums[w];
-        }
-        inc += off;
-        if (few) {
-            total = all;
-            run = run_places(total, a.runs);
-            v0 = run * blockIdx.x;
-            v1 = min(total, v0 + run);
-            if (v0 >= v1) return;  // the same for the whole CTA
-        }
-        if (l && inc > v0 && inc - l <= v0) {
-            found = s;
-            found_start = inc - l;
-        }
-        __syncthreads();
-        seg_start += all;
-        if (found >= 0) break;
+        places += seg_places(len);
     }
-    seg = found;
-    seg_start = found_start;
+    uint64_t off = places;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, off, o);
+        if (lane >= o) off += y;
+    }
+    if (lane == 31) sums[warp] = off;
+    __syncthreads();
+    off -= places;  // places before this thread's segments
+    uint64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) off += sums[w];
+        total += sums[w];
+    }
+    const uint64_t run = run_places(total, a.runs), v0 = run * blockIdx.x, v1 = min(total, v0 + run);
+    if (v0 >= v1) return;  // the same for the whole CTA
+    if (off <= v0 && v0 < off + places) {
+        int s = s0;
+        for (;; ++s) {
+            const uint64_t l = seg_places(kept ? len_s[s] : seg_len(a, s));
+            if (v0 < off + l) break;
+            off += l;
+        }
+        found = s;
+        found_start = off;
+    }
+    __syncthreads();
+    int seg = found;
+    uint64_t seg_start = found_start;  // places before it
 
     float slope[2] = {0.f, 0.f};
     if constexpr (BIAS) {
@@ -182,7 +178,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_step_kernel(const StepA
     }
 
     for (uint64_t at = v0; at < v1; ++seg) {
-        const uint64_t len = few ? len_s[seg] : seg_len(a, seg);
+        const uint64_t len = kept ? len_s[seg] : seg_len(a, seg);
         if (len == 0) continue;
         const uint64_t j0 = at - seg_start, j1 = min(len, v1 - seg_start);
         const bool entire = j0 == 0 && j1 == len;
@@ -191,7 +187,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_step_kernel(const StepA
             seg_start = at;
             continue;
         }
-        const uint64_t kbase = few ? begin_s[seg] : a.begin[seg];
+        const uint64_t kbase = kept ? begin_s[seg] : a.begin[seg];
         // Q as B fragments: head rr, the 8 columns 32 i + 8 qq of two reduction steps
         uint4 qf[2 * SETS];
 #pragma unroll

@@ -270,6 +270,13 @@ def test_step_many_cut_segments_odd_heads(G, dev):
     b.check(b.want())
 
 
+@pytest.mark.parametrize("n", [128, 129, 511, 512, 513, 1500])
+def test_step_segment_counts(G, dev, n):
+    b = Step(dev, [(7 * i) % 5 * ((i % 11) + 1) for i in range(n - 1)] + [900], 4, 2, 32, seed=n)
+    b.run_step(G)
+    b.check(b.want())
+
+
 def test_step_equals_the_last_row(G, dev):
     lens = [200, 1, 77]
     b = Batch(dev, lens, lens, 4, 2, 64, seed=1)
