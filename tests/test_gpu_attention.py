@@ -277,6 +277,17 @@ def test_step_segment_counts(G, dev, n):
     b.check(b.want())
 
 
+@pytest.mark.parametrize("heads,kv,dim,n", [(16, 4, 128, 300), (16, 16, 64, 90), (8, 2, 40, 777), (32, 1, 128, 200)])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (25.0, True)])
+def test_step_many_short_segments(G, dev, heads, kv, dim, n, cap, bias):
+    lens = [(13 * i) % 97 for i in range(n)]
+    lens[n // 2] = 3000  # one that many runs share
+    b = Step(dev, lens, heads, kv, dim, seed=n, gap=1)
+    sl = slopes_of(heads, dev) if bias else None
+    b.run_step(G, cap, sl)
+    b.check(b.want(cap=cap, slopes=sl))
+
+
 def test_step_equals_the_last_row(G, dev):
     lens = [200, 1, 77]
     b = Batch(dev, lens, lens, 4, 2, 64, seed=1)
