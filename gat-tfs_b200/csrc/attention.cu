@@ -788,6 +788,7 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                                          "r"(ou[6]), "r"(ou[7])
                                          : "memory");
                         }
+                        tmem_wait_st();  // the next such key reads the same columns
                     }
                 }
             }
