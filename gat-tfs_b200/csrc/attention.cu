@@ -543,10 +543,14 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
         const int hi_min = __reduce_min_sync(0xffffffffu, some ? hi : INT32_MAX);
         const int hi_max = __reduce_max_sync(0xffffffffu, some ? hi : 0);
         uint32_t met = 0;
+        // the other warp of the same rows has come as far, and its shared and tensor memory can be read
         auto meet_pair = [&] {
+            fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(pairs + 4 * tile + (warp & 3));
-            return mbar_wait_warp(pairs + 4 * tile + (warp & 3), met++ & 1u, abort_flag, &g_attention_error);
+            const bool met_it = mbar_wait_warp(pairs + 4 * tile + (warp & 3), met++ & 1u, abort_flag, &g_attention_error);
+            fence_after();
+            return met_it;
         };
         bool ok = true;
         uint32_t use = 0;
@@ -569,7 +573,10 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                 }
             };
             auto p_is_free = [&] {
-                return !kOwnP || use == 0 || mbar_wait_warp(pv_done, (use - 1) & 1u, abort_flag, &g_attention_error);
+                if (!kOwnP || use == 0) return true;
+                const bool done = mbar_wait_warp(pv_done, (use - 1) & 1u, abort_flag, &g_attention_error);
+                fence_after();
+                return done;
             };
             if constexpr (FIXED) {
                 WeightSum sum;

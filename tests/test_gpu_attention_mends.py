@@ -4,7 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import attention_reference as R  # noqa: E402
-from test_gpu_attention import Batch  # noqa: E402
+from test_gpu_attention import Batch, slopes_of  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,36 @@ def test_many_non_finite_values_of_a_block(G, dev, dim, mask):
     prefix = [20, 99, 45] if mask == 2 else None
     b.run(G, mask, prefix)
     b.check(b.reference(mask=mask, prefix=prefix))
+
+
+@pytest.mark.parametrize("cap,bias", [(20.0, False), (50.0, False), (20.0, True), (50.0, True), (60.0, True), (0.0, True)])
+@pytest.mark.parametrize("mask", [0, 1, 2])
+@pytest.mark.parametrize("dim", [40, 128])
+def test_many_non_finite_values_under_caps_and_biases(G, dev, dim, mask, cap, bias):
+    lens = [30, 100, 90]
+    b = Batch(dev, lens, lens, 4, 2, dim, seed=dim, qscale=4.0)
+    plant(b)
+    prefix = [20, 99, 45] if mask == 2 else None
+    sl = slopes_of(4, dev) if bias else None
+    b.run(G, mask, prefix, cap, sl)
+    b.check(b.reference(mask=mask, prefix=prefix, cap=cap, slopes=sl))
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -3.3e38])
+@pytest.mark.parametrize("cap,bias", [(20.0, False), (50.0, True)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_what_is_masked_never_arrives_under_a_cap(G, dev, value, cap, bias, dim):
+    """Segments and earlier rows beside non-finite keys and values, to the tolerance: the polynomial of the tanh is
+    chosen by a block's products, masked ones among them, so the last bits may differ."""
+    lens = [30, 100, 60, 200, 129]
+    b = Batch(dev, lens, lens, 2, 2, dim, seed=5)
+    sl = slopes_of(2, dev) if bias else None
+    want = b.reference(mask=1, cap=cap, slopes=sl)
+    b.k[40, :dim] = value
+    b.v[45, 3] = value
+    b.v[300, 10:30] = value
+    b.q[200, 5] = value
+    b.run(G, 1, None, cap, sl)
+    rows = torch.tensor([i for s in (0, 2, 4) for i in range(b.q_row[s], b.q_row[s + 1])] + list(range(30, 40)) +
+                        [i for i in range(190, 300) if i != 200], device=dev)
+    R.check(b.out[rows, :2 * dim], b.lse[rows], {key: t[rows] for key, t in want.items()})
