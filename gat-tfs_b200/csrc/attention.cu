@@ -30,10 +30,13 @@
 // takes the tensor cores as long as its exponentials): the cap's tanh is a
 // polynomial on the FMA pipe wherever a block's scores stay below 0.6 cap. A
 // row's largest capped score lies within +-cap (of the bias of its nearest key),
-// so up to a cap of 55 the weights are taken relative to cap / 2 (and that bias)
-// instead of the running maximum (the largest is 2^-120 .. 2^40, an ordinary FP32
-// and BF16 number): no pass for the maximum, no rescaling, 32 columns at a time
-// flow from S to P and two threads share a row. (With a maximum to agree on, two
+// so up to a cap of 55 the weights are taken relative to cap / 4 (and that bias)
+// instead of the running maximum. The largest weight of a row is then 2^-100 ..
+// 2^60, so that in the lowest of rows a key counts until it is 2^-26 of the
+// largest one (what a bias pushes further down is flushed to zero at 2^-126, less
+// than 2e-6 of the row's sum) and values from 2^-26 to 2^40 keep their products
+// among FP32's ordinary numbers. No pass for the maximum, no rescaling, 32 columns
+// at a time flow from S to P and two threads share a row. (With a maximum to agree on, two
 // threads a row were slower than one: 8192 x 32 x 128 causal, 320 us and 359 us.)
 #include <cuda.h>
 
@@ -184,7 +187,7 @@ __device__ __forceinline__ uint32_t visible(int b, int e) {
 
 // Growth of the maximum (log2) up to which the reference stays.
 constexpr float kGrow = 24.f;
-// Largest cap * log2 e whose weights are taken relative to half of it.
+// Largest cap * log2 e whose weights are taken relative to a quarter of it.
 constexpr float kFixedCap = 80.f;
 // The polynomials' coefficients take scale / cap into themselves, in powers up
 // to the ninth: used for scale / cap up to kTanhScale and products q.k whose
@@ -193,7 +196,7 @@ constexpr double kTanhScale = 8192.0;
 constexpr float kTanhProducts = 4915.f;
 
 // DP: dim rounded up to 64 or 128. CAP / BIAS: scores go through the tanh / get the distance bias.
-// FIXED: weights relative to half the cap (capped scores).
+// FIXED: weights relative to a quarter of the cap (capped scores).
 // TMEM, one tile: S at 0, P at 128, O at 192; two: S and P of tile t at 128 t, O at 256 + 128 t.
 template <int DP, bool FIXED>
 struct Shape {
@@ -529,7 +532,7 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
             for (int i = 0; i < 3; ++i) tk3[i] = FIXED ? pair_of(g.tanh3[i]) : 0;
         }
         // the reference maximum (log2 units), the sums of the weights and of the rounded weights
-        float m = FIXED ? 0.5f * g.zcap : -INFINITY, l = 0.f, lr = 0.f;
+        float m = FIXED ? 0.25f * g.zcap : -INFINITY, l = 0.f, lr = 0.f;
         // FIXED with a bias: the distance of the row's nearest key (farthest with a negative slope), whose
         // bias the weights are relative to
         const int past = pos - (hi - lo - 1);  // behind the last key that it sees

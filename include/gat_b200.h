@@ -365,7 +365,10 @@ int gat_b200_aggregate_fused_noalloc(uint64_t n, uint64_t e, const uint64_t* row
  * rows 16-byte aligned. lse: FP32 [n_q][heads] or NULL. slopes: FP32 [heads].
  * dim: a multiple of 8, at most 128 (GAT_B200_EUNSUPPORTED otherwise). scale in
  * (0, 1e30], cap in [0, 1e30]. Scores
- * and sums are FP32; the weights are rounded to BF16 for the second product. */
+ * and sums are FP32; the weights are rounded to BF16 for the second product, and
+ * taken relative to a fixed score (cap up to 55) or to a maximum that follows
+ * slowly: magnitudes of v above 2^40 may overflow to Inf, and in rows whose
+ * scores all lie near -cap, cap above 40, those below 2^-26 lose bits. */
 int gat_b200_masked_attention(int heads, int kv_heads, int dim, int nseg, uint64_t n_q, uint64_t n_k,
                               const uint64_t* q_row, const uint64_t* k_row, int mask,
                               const uint64_t* prefix, const void* q, int ldq, const void* k, int ldk,

@@ -67,3 +67,29 @@ def test_what_is_masked_never_arrives_under_a_cap(G, dev, value, cap, bias, dim)
     rows = torch.tensor([i for s in (0, 2, 4) for i in range(b.q_row[s], b.q_row[s + 1])] + list(range(30, 40)) +
                         [i for i in range(190, 300) if i != 200], device=dev)
     R.check(b.out[rows, :2 * dim], b.lse[rows], {key: t[rows] for key, t in want.items()})
+
+
+@pytest.mark.parametrize("cap", [30.0, 50.0, 53.0, 55.0, 55.4, 56.0])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_saturated_scores_under_a_bias(G, dev, cap, sign, dim):
+    """All scores lie at -cap (or cap), so the bias alone decides: keys far below the nearest one's weight still count."""
+    lens = [1500, 40]
+    for slopes in ([0.5, 2.0 ** -8, -0.5, -2.0 ** -8], [3.0, 2.0 ** -6, 0.0, 2.0 ** -10]):
+        b = Batch(dev, lens, lens, 4, 2, dim, seed=3)
+        b.q[:b.nq, :4 * dim], b.k[:b.nk, :2 * dim] = 8.0, sign * 8.0
+        sl = torch.tensor(slopes, device=dev)
+        for mask in (0, 1):
+            b.run(G, mask, None, cap, sl)
+            b.check(b.reference(mask=mask, cap=cap, slopes=sl))
+
+
+@pytest.mark.parametrize("cap", [30.0, 55.4, 56.0])
+@pytest.mark.parametrize("sign,size", [(-1.0, 2.0 ** -20), (-1.0, 1.0), (1.0, 1.0), (1.0, 2.0 ** 40)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_saturated_scores_and_the_size_of_values(G, dev, cap, sign, size, dim):
+    b = Batch(dev, [300, 1], [300, 1], 2, 1, dim, seed=3)
+    b.q[:b.nq, :2 * dim], b.k[:b.nk, :dim] = 8.0, sign * 8.0
+    b.v *= size
+    b.run(G, 1, None, cap)
+    b.check(b.reference(mask=1, cap=cap))
