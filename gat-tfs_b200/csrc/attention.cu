@@ -613,8 +613,10 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                         continue;
                     }
                     const float rel = float(pos + jl - 32 * w);  // distance of column c: |rel - c|
-                    const bool before = BIAS && __all_sync(0xffffffffu, rel >= 31.f);
-                    const float off = before ? fmaf(nslope, rel - near, -m) : -m;
+                    // all columns before the rows: the last one's bias and, per column, what it has more (both
+                    // of one sign, so that a near key does not carry the rounding of a far one's bias)
+                    const bool before = BIAS && nslope <= 0.f && __all_sync(0xffffffffu, rel >= 31.f);
+                    const float off = before ? fmaf(nslope, rel - 31.f - near, -m) : -m;
                     const f32x2 nref = pack2(off, off);
                     if (degree == 3) {
 #pragma unroll
@@ -639,7 +641,7 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                     }
                     if (before) {
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) x[c] = fmaf(float(-c), nslope, x[c]);
+                        for (int c = 0; c < 32; ++c) x[c] = fmaf(float(31 - c), nslope, x[c]);
                     } else if (BIAS) {
 #pragma unroll
                         for (int c = 0; c < 32; ++c) x[c] = fmaf(nslope, fabsf(rel - float(c)) - near, x[c]);
@@ -690,10 +692,11 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                 const float rel = float(pos + jl);  // distance of column c: |rel - c|
                 // (with a cap as well there are no registers to spare for the shorter form)
                 if (!CAP && __all_sync(0xffffffffu, rel >= float(kRows - 1))) {
-                    const float base = nslope * rel;
+                    // as above: the last column's bias and what the others have more
+                    const float base = nslope * (rel - float(kRows - 1));
 #pragma unroll
                     for (int c = 0; c < kRows; ++c) {
-                        const float e = fmaf(float(-c), nslope, base);
+                        const float e = fmaf(float(kRows - 1 - c), nslope, base);
                         z[c] = fmaf(z[c], g.zscale, e);
                     }
                 } else {

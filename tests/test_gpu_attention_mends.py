@@ -93,3 +93,37 @@ def test_saturated_scores_and_the_size_of_values(G, dev, cap, sign, size, dim):
     b.v *= size
     b.run(G, 1, None, cap)
     b.check(b.reference(mask=1, cap=cap))
+
+
+def lse_of(z):
+    """log-sum-exp per row of FP64 scores [rows][keys] (-inf: not seen) and each key's share of its row."""
+    lse = torch.logsumexp(z, 1)
+    return lse, torch.exp(z - lse[:, None]).nan_to_num(0.0)
+
+
+@pytest.mark.parametrize("cap", [0.0, 30.0, 60.0])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("slope", [1.0, 64.0, 1000.0, 1e6, -64.0, -1e6])
+@pytest.mark.parametrize("mask", [0, 1])
+def test_steep_biases_keep_the_score(G, dev, cap, dim, slope, mask):
+    """The bias of the key that decides a row may not carry the rounding of a larger one: at distance 0 a score stays what
+    it is, whatever the slope."""
+    first, n = 97, 403  # the second segment begins inside a tile, so that blocks end at every row of a warp
+    b = Batch(dev, [first, n], [first, n], 1, 1, dim, seed=4, qscale=2.0)
+    sl = torch.tensor([slope], device=dev)
+    b.run(G, mask, None, cap, sl)
+    q, k = b.q[first:first + n, :dim].double(), b.k[first:first + n, :dim].double()
+    dot, mag = q @ k.t() * b.scale, q.abs() @ k.abs().t() * b.scale
+    z = cap * torch.tanh(dot / cap) if cap else dot
+    far = (torch.arange(n, device=dev)[:, None] - torch.arange(n, device=dev)[None, :])
+    seen = far >= 0 if mask else far > -n
+    far = far.abs().double()
+    # FP32: dim products and sums, the coefficients' and the tanh's error, four roundings of the score (with the
+    # reference that is taken off, a quarter of the cap), two of the key's own bias; shared out by the keys' weights
+    err = mag * (dim + 4) * 2.0 ** -24 + (z.abs() + cap / 4) * 2.0 ** -21 + abs(slope) * far * 2.0 ** -22
+    z = torch.where(seen, z - slope * far, torch.full_like(z, -float("inf")))
+    lse, w = lse_of(z)
+    # then the sum's logarithm and the reference added to it
+    tol = 2 * (w * err).sum(1) + 2.0 ** -20 + (lse.abs() + cap) * 2.0 ** -22 + n * 2.0 ** -24
+    over = (b.lse[first:first + n, 0].double() - lse).abs() / tol
+    assert float(over.max()) <= 1, float(over.max())
