@@ -14,6 +14,10 @@
 // slots a column takes does not matter as long as q and k agree):
 //   S^T [16 keys x 8 heads] = K Q^T;  P^T by movmatrix;  O^T [16 columns x 8 heads] += V^T P^T.
 // mma.sync is ample: 16 keys are 16 MMAs for 8 KB of K and V.
+//
+// P is rounded to BF16 (the MMA's input type). A warp's weighted values are an
+// average over its own rounded weights, scaled to the sum of the unrounded ones,
+// with which states are joined and the log-sum-exp is made.
 #include "attention.cuh"
 
 namespace gatb {
@@ -198,7 +202,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_step_kernel(const StepA
         float o[kTiles][4];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, lr[2] = {0.f, 0.f};  // maximum, sums of weights and rounded weights
 
         for (uint64_t j = j0 + warp * kKeys; j < j1; j += kWarps * kKeys) {
             const uint16_t* kp = a.k + (kbase + j) * uint64_t(a.ldk) + uint64_t(kvh) * a.dim;
@@ -270,6 +274,8 @@ __global__ void __launch_bounds__(kWarps * 32) attention_step_kernel(const StepA
                 }
                 l[0] *= f[0];
                 l[1] *= f[1];
+                lr[0] *= f[0];
+                lr[1] *= f[1];
                 m[0] = mn[0];
                 m[1] = mn[1];
             }
@@ -282,7 +288,10 @@ __global__ void __launch_bounds__(kWarps * 32) attention_step_kernel(const StepA
                     p[e] = ex2(z[t][e] - ref[e & 1]);
                     l[e & 1] += p[e];
                 }
-                const uint32_t b0 = transpose8x8(pack_bf16x2(p[0], p[1])), b1 = transpose8x8(pack_bf16x2(p[2], p[3]));
+                const uint32_t r0 = pack_bf16x2(p[0], p[1]), r1 = pack_bf16x2(p[2], p[3]);
+                lr[0] += bf16lo(r0) + bf16lo(r1);
+                lr[1] += bf16hi(r0) + bf16hi(r1);
+                const uint32_t b0 = transpose8x8(r0), b1 = transpose8x8(r1);
 #pragma unroll
                 for (int s = 0; s < SETS; ++s) {
                     const uint32_t* x0 = &vf[t][0][s].x;
@@ -304,7 +313,11 @@ __global__ void __launch_bounds__(kWarps * 32) attention_step_kernel(const StepA
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
-            for (int s = 4; s < 32; s <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], s);
+            for (int s = 4; s < 32; s <<= 1) {
+                l[i] += __shfl_xor_sync(0xffffffffu, l[i], s);
+                lr[i] += __shfl_xor_sync(0xffffffffu, lr[i], s);
+            }
+            const float own = lr[i] > 0.f ? l[i] / lr[i] : 1.f;  // no weights: zeros
             if (rr == 0) {
                 m_s[warp][2 * qq + i] = m[i];
                 l_s[warp][2 * qq + i] = l[i];
@@ -312,8 +325,8 @@ __global__ void __launch_bounds__(kWarps * 32) attention_step_kernel(const StepA
 #pragma unroll
             for (int t = 0; t < kTiles; ++t) {
                 const int col = 64 * (t >> 2) + 8 * rr + 2 * (t & 3);
-                o_s[warp][2 * qq + i][col] = o[t][i];
-                o_s[warp][2 * qq + i][col + 1] = o[t][2 + i];
+                o_s[warp][2 * qq + i][col] = o[t][i] * own;
+                o_s[warp][2 * qq + i][col + 1] = o[t][2 + i] * own;
             }
         }
         __syncthreads();

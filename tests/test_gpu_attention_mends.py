@@ -1,10 +1,12 @@
 """Masked attention where it is easily wrong: several non-finite values in a block, steep biases, caps that
 saturate, rows outside the segments. Against the FP64 definition (attention_reference.py)."""
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
 import attention_reference as R  # noqa: E402
-from test_gpu_attention import Batch, slopes_of  # noqa: E402
+from test_gpu_attention import Batch, Step, slopes_of  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -127,3 +129,24 @@ def test_steep_biases_keep_the_score(G, dev, cap, dim, slope, mask):
     tol = 2 * (w * err).sum(1) + 2.0 ** -20 + (lse.abs() + cap) * 2.0 ** -22 + n * 2.0 ** -24
     over = (b.lse[first:first + n, 0].double() - lse).abs() / tol
     assert float(over.max()) <= 1, float(over.max())
+
+
+@pytest.mark.parametrize("lens", [[1000], [40, 3, 0, 700], [20000], [9, 5000, 300]])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_step_of_equal_values_is_that_value(G, dev, lens, dim):
+    """A row is an average over its own rounded weights: here all weights but one round down by nearly half a step, and a
+    constant column still comes out as it is."""
+    b = Step(dev, lens, 4, 2, dim, seed=1)
+    b.q[:, :4 * dim], b.k[:b.nk, :2 * dim] = 0, 0
+    b.q[:b.nq, 0:4 * dim:dim], b.k[:b.nk, 0:2 * dim:dim] = 1.0, -1.0
+    for s, n in enumerate(lens):
+        if n:
+            b.k[b.begin[s] + n // 2, :2 * dim] = 0.0  # the largest weight, 1
+    b.scale = -math.log(0.5 * (1 + 0.0035))
+    value = (1 + torch.arange(2 * dim, device=dev) / (2 * dim)).to(torch.bfloat16)
+    b.v[:b.nk, :2 * dim] = value
+    b.run_step(G)
+    want = value.view(2, 1, dim).expand(2, 2, dim).reshape(-1)
+    for s, n in enumerate(lens):
+        assert torch.equal(b.out[s, :4 * dim], want if n else torch.zeros_like(want)), s
+    b.check(b.want())
