@@ -88,6 +88,19 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar) {
         : "memory");
 }
 
+// A sum v times two row scales a and b may well be an FP32 number where a b is
+// none (rows of huge or tiny elements). NVFP4's v is zero or at least 2^-20
+// (products of block scales and elements), at most 2^23 k, so ((v first) b) rest
+// with a = first * rest, rest a power of two, leaves FP32's range only where the
+// result does. (MXFP4's block scales span FP32's range by themselves.)
+__device__ __forceinline__ bool ordinary(float x) { return fabsf(x) >= 0x1p-50f && fabsf(x) <= 0x1p50f; }
+__device__ __forceinline__ float split_scale(float a, float& rest) {
+    const float m = fabsf(a);
+    const bool huge = m > 0x1p80f, tiny = m < 0x1p-100f;
+    rest = huge ? 0x1p40f : tiny ? 0x1p-50f : 1.f;
+    return a * (huge ? 0x1p-40f : tiny ? 0x1p50f : 1.f);
+}
+
 // ------------------------------------------------------------ CTA pairs
 // Roles of the 20 warps of each CTA of a pair (2 and 3 idle):
 //   warp 0    TMA producer: this CTA's 128 rows of a, 128 of the tile's 256 rows
@@ -233,7 +246,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         uint8_t* sb = st_s + ew * 4096;
         float* rb = rb_s + ew * 64;
         // the row scales of a tile, fetched while the one before it is worked on
-        float ra = 1.f, rb0 = 0.f, rb1 = 0.f;
+        float ra = 1.f, rb0 = 1.f, rb1 = 1.f;
         uint32_t tm = 0, tn = 0;
         auto fetch = [&](uint32_t t) {
             tile_at(t, tm, tn);
@@ -250,6 +263,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             const uint64_t row0 = uint64_t(tm) * 256 + rank * 128 + q * 32;
             const int col = int(tn) * 256 + grp * 64;
             const float ra_t = ra;
+            // outside the usual range of scales the tile takes them one after the other
+            const bool wild = __any_sync(0xffffffffu, !ordinary(ra) || !ordinary(rb0) || !ordinary(rb1));
             __syncwarp();  // the last tile's reads of rb
             rb[lane] = rb0;
             rb[lane + 32] = rb1;
@@ -263,7 +278,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive_rank(drained, 0);
             if (col >= g.n || row0 >= g.m) continue;
-            if (g.b_row) {
+            if (wild && g.b_row) {
+                float rest;
+                const float first = split_scale(ra_t, rest);
+#pragma unroll
+                for (int c = 0; c < 64; ++c) v[c] = v[c] * first * rb[c] * rest;
+            } else if (g.b_row) {
 #pragma unroll
                 for (int c = 0; c < 64; c += 4) {
                     const float4 b4 = *reinterpret_cast<const float4*>(rb + c);
@@ -506,9 +526,10 @@ __global__ void __launch_bounds__(kRowsThreads)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[e] += x[e];
             }
-            const float ra = ra_s[r];
+            float rest;
+            const float ra = split_scale(ra_s[r], rest);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] *= ra * rb_s[c + e];
+            for (int e = 0; e < 4; ++e) y[e] = y[e] * ra * rb_s[c + e] * rest;
             const uint64_t off = (arow + r) * uint64_t(g.ldo) + col;
             if (g.out_bf16) {
                 uint16_t* o = static_cast<uint16_t*>(g.out) + off;
