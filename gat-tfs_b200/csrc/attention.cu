@@ -295,14 +295,14 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
     const int tile = kTiles == 2 && warp >= 4 + 4 * kHalves ? 1 : 0;
     const int r = (warp & 3) * 32 + lane;
     const uint64_t row = row0 + uint64_t(tile) * kRows + r;
-    int lo = 0, hi = 0, pos = 0;
+    int lo = 0, hi = -1, pos = 0;  // hi -1: no row, or one outside the segments
     if (warp >= 4) {
         const int s = segment_of_lane(g.q_row, g.nseg, row - lane, lane);
-        if (row < g.n_q) {
-            // row pointers are taken as given but kept inside the tables
-            const uint64_t q0 = g.q_row[s], q1 = g.q_row[s + 1];
+        // row pointers are taken as given but kept inside the tables
+        const uint64_t q0 = g.q_row[s], q1 = g.q_row[s + 1];
+        if (row < g.n_q && row >= q0 && row < q1) {
             const uint64_t ks = min(g.k_row[s], g.n_k), ke = max(ks, min(g.k_row[s + 1], g.n_k));
-            const int64_t at = int64_t(row - min(q0, row)) + int64_t(ke - ks) - int64_t(max(q1, q0) - q0);
+            const int64_t at = int64_t(row - q0) + int64_t(ke - ks) - int64_t(q1 - q0);
             lo = int(ks);
             hi = int(ke);
             if (g.mask != GAT_B200_MASK_FULL) {
@@ -821,7 +821,7 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
                 lr = s2[2 * kRows + r] + s2[3 * kRows + r];
             }
             const float inv = hi > lo ? 1.f / lr : 0.f;
-            const bool live = row < g.n_q;
+            const bool live = hi >= 0;
             uint16_t* orow = g.out + row * uint64_t(g.ldo) + uint64_t(head) * g.dim + kOCols * half;
 #pragma unroll 1
             for (int c = 0; c < kOCols; c += 32) {
@@ -843,7 +843,7 @@ __global__ void __launch_bounds__(Shape<DP, FIXED>::kThreads, Shape<DP, FIXED>::
             if (live && g.lse && half == 0) g.lse[row * g.heads + head] = hi > lo ? ((FIXED && BIAS ? fmaf(nslope, near, m) : m) + log2f(l)) * kLn2 : -INFINITY;
         }
     }
-    if (my_to == 0 && row < g.n_q && half == 0) {  // every row of the tile sees nothing
+    if (my_to == 0 && hi >= 0 && half == 0) {  // every row of the tile sees nothing
         uint16_t* orow = g.out + row * uint64_t(g.ldo) + uint64_t(head) * g.dim;
         for (int c = 0; c < g.dim; c += 8) *reinterpret_cast<uint4*>(orow + c) = make_uint4(0, 0, 0, 0);
         if (g.lse) g.lse[row * g.heads + head] = -INFINITY;

@@ -354,8 +354,9 @@ int gat_b200_aggregate_fused_noalloc(uint64_t n, uint64_t e, const uint64_t* row
  *           - slopes[h] * |position of i - j|    (slopes NULL: no bias)
  *   out_i = sum_j exp(z_ij) v_j / sum_j exp(z_ij),  lse_i = log sum_j exp(z_ij)
  * Rows q_row[s] .. q_row[s+1] and keys k_row[s] .. k_row[s+1] (device, uint64
- * [nseg+1], as a CSR's row pointers: q_row[0] = 0, q_row[nseg] = n_q,
- * non-decreasing) belong to segment s; a segment may have no rows or no keys.
+ * [nseg+1], non-decreasing as a CSR's row pointers) belong to segment s; a
+ * segment may have no rows or no keys. Rows outside all segments, such as those
+ * behind the last one in a padded batch, keep what out and lse held.
  * Like the CSR of gat_b200_aggregate_fused_noalloc they are read as given, but
  * kept inside n_q and n_k. prefix: device uint64 [nseg], MASK_PREFIX only.
  * A row that sees no key gets zeros and lse -inf. What a row does not see never

@@ -150,3 +150,20 @@ def test_step_of_equal_values_is_that_value(G, dev, lens, dim):
     for s, n in enumerate(lens):
         assert torch.equal(b.out[s, :4 * dim], want if n else torch.zeros_like(want)), s
     b.check(b.want())
+
+
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (30.0, True)])
+@pytest.mark.parametrize("mask", [0, 1])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_row", [[0, 60, 150, 200], [0, 0, 0, 0], [10, 60, 130, 131], [0, 128, 128, 256], [0, 300, 700, 700]])
+def test_rows_outside_the_segments_are_left_alone(G, dev, q_row, dim, mask, cap, bias):
+    """A padded batch: fewer rows in the segments than in the table, the rest as they were."""
+    b = Batch(dev, [300, 300, 100], [70, 300, 40], 2, 1, dim, seed=11)
+    b.q_row = q_row
+    sl = slopes_of(2, dev) if bias else None
+    b.run(G, mask, None, cap, sl)
+    first, last = q_row[0], q_row[-1]
+    want = b.reference(mask=mask, cap=cap, slopes=sl)
+    R.check(b.out[first:last, :2 * dim], b.lse[first:last], {key: t[first:last] for key, t in want.items()})
+    for t in (b.out, b.lse):
+        assert (t[:first] == -7).all() and (t[last:] == -7).all()
