@@ -167,3 +167,33 @@ def test_rows_outside_the_segments_are_left_alone(G, dev, q_row, dim, mask, cap,
     R.check(b.out[first:last, :2 * dim], b.lse[first:last], {key: t[first:last] for key, t in want.items()})
     for t in (b.out, b.lse):
         assert (t[:first] == -7).all() and (t[last:] == -7).all()
+
+
+@pytest.mark.parametrize("part", [0.01, 0.1, 0.199, 0.201, 0.29, 0.599, 0.601, 0.9, 3.0])
+@pytest.mark.parametrize("cap", [5.0, 30.0, 55.0, 60.0])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_capped_scores_to_a_few_roundings(G, dev, cap, dim, part):
+    """Rows of one key, whose log-sum-exp is the capped score itself, with the largest score of a block on either side of
+    the polynomials' limits (0.2 and 0.6 of the cap)."""
+    n = 512
+    b = Batch(dev, [1] * n, [1] * n, 1, 1, dim, seed=1)
+    b.q[:n, :dim], b.k[:n, :dim] = 0, 0
+    b.q[:n, 0] = 1.0
+    top = torch.tensor(part * cap).to(torch.bfloat16).float()
+    b.k[:n, 0] = (top.to(dev) * torch.linspace(-1, 1, n, device=dev)).to(torch.bfloat16)
+    b.k[:n:32, 0] = top.to(dev).to(torch.bfloat16)
+    b.scale = 1.0
+    dot = b.k[:n, 0].double()
+    z = cap * torch.tanh(dot / cap)
+    # relative to z, in units of 2^-24: the polynomial 2 (1.2e-7), its coefficients and steps 5, the last product with
+    # log2 e 2, the end 1; the tanh by ex2 and rcp (2^-22 and 2^-23 of their own) 6 more. Relative to |z| + cap / 4, as
+    # the weight is relative to a quarter of the cap: its exponent, its logarithm (1 step), their sum. And ex2 itself.
+    tol = (z.abs() * (10 if part < 0.6 else 16) + (z.abs() + cap / 4) * 4) * 2.0 ** -24 + 2.0 ** -21
+    b.run(G, 0, None, cap, None)
+    over = (b.lse[:n, 0].double() - z).abs() / tol
+    assert float(over.max()) <= 1, float(over.max())
+    s = Step(dev, [1] * n, 1, 1, dim, seed=1)
+    s.q, s.k, s.scale = b.q, b.k, 1.0
+    s.run_step(G, cap)
+    over = (s.lse[:n, 0].double() - z).abs() / tol
+    assert float(over.max()) <= 1, float(over.max())
