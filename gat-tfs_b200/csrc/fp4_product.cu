@@ -110,12 +110,13 @@ __device__ __forceinline__ float split_scale(float a, float& rest) {
 //   warps 4-19 epilogue: 32 rows x 64 columns of this CTA's 128 x 256
 //             accumulators each, in registers at once, so the next tile's MMAs
 //             start while this one is scaled, rounded and stored.
-// Tensor memory: accumulators of even tiles in columns 0-255, of odd tiles in
-// 192-447, scales in 448-511 (two whole accumulators and the scales do not fit).
+// Tensor memory: accumulators in columns 0-255, scales in 448-511 (two whole
+// accumulators and the scales do not fit): a tile's MMAs wait until all epilogue
+// warps have the one before it in registers.
 constexpr int kEpiWarps = 16;
 constexpr int kPairThreads = 128 + 32 * kEpiWarps;
 constexpr int kPairStages = 4;
-constexpr int kOdd = 192, kScaleCols = 448;
+constexpr int kScaleCols = 448;
 
 template <int FORMAT>
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
@@ -133,8 +134,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(rb_s + kEpiWarps * 64);
     uint64_t* full = bars;
     uint64_t* empty = full + kPairStages;
-    uint64_t* acc_full = empty + kPairStages;  // [2]
-    uint64_t* drained = acc_full + 2;
+    uint64_t* acc_full = empty + kPairStages;
+    uint64_t* drained = acc_full + 1;
     uint64_t* mma_done = drained + 1;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(mma_done + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
@@ -155,8 +156,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             mbar_init(full + s, 1);
             mbar_init(empty + s, 1);
         }
-        mbar_init(acc_full + 0, 1);
-        mbar_init(acc_full + 1, 1);
+        mbar_init(acc_full, 1);
         mbar_init(drained, 2 * kEpiWarps);
         mbar_init(mma_done, 1);
         *abort_flag = 0;
@@ -207,7 +207,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             for (uint32_t t = pair; t < ntiles && ok; t += pairs, ++tl) {
                 if (tl && !mbar_wait_warp(drained, (tl - 1) & 1u, abort_flag, &g_fp4_error)) { ok = false; break; }
                 fence_after();
-                const uint32_t d = tmem + ((tl & 1u) ? kOdd : 0);
                 for (int k = 0; k < g.stages_k; ++k, ++kc) {
                     const int s = int(kc % kPairStages);
                     if (!mbar_wait_warp(full + s, (kc / kPairStages) & 1u, abort_flag, &g_fp4_error)) { ok = false; break; }
@@ -228,12 +227,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
                                 tmem_cp_scales<2>(sfb, fdesc + S::kBytes / 16 + st * 32);
                                 tmem_cp_scales<2>(sfb + 4, fdesc + 2 * S::kBytes / 16 + st * 32);
                             }
-                            mma_fp4<S::kMx, 2>(d, adesc + j * 2, bdesc + j * 2,
+                            mma_fp4<S::kMx, 2>(tmem, adesc + j * 2, bdesc + j * 2,
                                                idesc_fp4(256, 256, S::kMx, S::kMx ? 2 * (j & 1) : 0), sfa, sfb,
                                                (k | j) ? 1u : 0u);
                         }
                         pair_commit(empty + s);
-                        if (k + 1 == g.stages_k) pair_commit(acc_full + (tl & 1u));
+                        if (k + 1 == g.stages_k) pair_commit(acc_full);
                     }
                     __syncwarp();
                 }
@@ -259,7 +258,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         if (pair < ntiles) fetch(pair);
         uint32_t tl = 0;
         for (uint32_t t = pair; t < ntiles; t += pairs, ++tl) {
-            const uint32_t odd = tl & 1u;
             const uint64_t row0 = uint64_t(tm) * 256 + rank * 128 + q * 32;
             const int col = int(tn) * 256 + grp * 64;
             const float ra_t = ra;
@@ -270,10 +268,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             rb[lane + 32] = rb1;
             __syncwarp();
             if (t + pairs < ntiles) fetch(t + pairs);
-            if (!mbar_wait_warp(acc_full + odd, (tl >> 1) & 1u, abort_flag, &g_fp4_error)) break;
+            if (!mbar_wait_warp(acc_full, tl & 1u, abort_flag, &g_fp4_error)) break;
             fence_after();
             float v[64];
-            tmem_ld64(tmem + (odd ? kOdd : 0) + (uint32_t(q * 32) << 16) + grp * 64, v);
+            tmem_ld64(tmem + (uint32_t(q * 32) << 16) + grp * 64, v);
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_rank(drained, 0);
