@@ -894,6 +894,7 @@ int attention_check(const char* what, const AttentionShape& s, uint64_t n_q, uin
     if (s.dim <= 0 || s.dim > 128 || s.dim % 8) return fail_code(GAT_B200_EUNSUPPORTED, w + "dim must be a multiple of 8, at most 128");
     if (n_q > uint64_t(INT32_MAX - 512) || n_k > uint64_t(INT32_MAX - 512)) return fail(w + "too many rows");
     if (nseg < 0) return fail(w + "bad segment count");
+    if (nseg > INT32_MAX - 513) return fail(w + "too many segments");
     if (!(s.scale > 0.f) || s.scale > 1e30f) return fail(w + "scale must be positive, at most 1e30");
     if (!(s.cap >= 0.f) || s.cap > 1e30f) return fail(w + "cap must lie in 0 (none) .. 1e30");
     if (s.cap > 0.f && s.scale / s.cap > 1e30f) return fail(w + "cap too small for the scale");
