@@ -255,8 +255,8 @@ __device__ __forceinline__ float reciprocal_e4m3(float s) {
 // x or rows of the values are not all whole, aligned fours of elements.
 // Issue slots bind it as much as memory does, hence packed FP32 pairs and no
 // branches on alignment inside: 2,449,029 x 100 FP32 to NVFP4 with BF16 values
-// took 389 us with scalar arithmetic and such branches and takes 294 us
-// (5.5 TB/s); 169,343 x 128 FP32 to MXFP4 25 us (5.6 TB/s).
+// took 389 us with scalar arithmetic and such branches and takes 318 us
+// (5.1 TB/s); 169,343 x 128 FP32 to MXFP4 26.5 us (5.3 TB/s).
 template <int FORMAT, bool BF16, bool LOOSE, int LANES, int CHUNKS, bool REREAD>
 __global__ void __launch_bounds__(256) fp4_quantize_kernel(const QuantArgs a) {
     constexpr bool kNv = FORMAT == GAT_B200_NVFP4;

@@ -262,7 +262,8 @@ uint64_t gat_b200_fp4_scale_bytes(int format, uint64_t n, int width);
  * are those of the exact quotients. A block (MXFP4) or row (NVFP4) with an Inf
  * or NaN gets a NaN scale: all of it reads as NaN. If values is not NULL, what
  * the table stands for is written there (FP32 or BF16, [n][ldv]; exact in
- * both, but for magnitudes below the type's normal range). Scale bytes of rows
+ * both, but for magnitudes below the type's normal range, and Inf for the few
+ * above its range that elements near 3.4e38 can round to). Scale bytes of rows
  * past n are left as they were. x and what is written do not overlap. */
 int gat_b200_fp4_quantize(int format, uint64_t n, int width, const void* x, int x_dtype, int ldx,
                           void* codes, int ldc, void* scales, float* row_scale, void* values,
@@ -273,7 +274,9 @@ int gat_b200_fp4_quantize(int format, uint64_t n, int width, const void* x, int 
  * weights), FP32 accumulation on the 4-bit tensor cores, times a_row[i] and
  * b_row[j] (FP32, NULL = 1), rounded to out_dtype (FP32 or BF16), [m][ldo].
  * lda / ldb: bytes per code row. Columns of out behind n are left as they
- * were. */
+ * were. Row scales of NVFP4 may be any FP32 numbers: with k up to 131,072 only
+ * a result outside FP32's range overflows or underflows. out overlaps none of
+ * the inputs. */
 int gat_b200_fp4_product(int format, uint64_t m, int n, int k, const void* a, int lda,
                          const void* a_scales, const float* a_row, const void* b, int ldb,
                          const void* b_scales, const float* b_row, void* out, int out_dtype, int ldo,
@@ -364,7 +367,8 @@ int gat_b200_aggregate_fused_noalloc(uint64_t n, uint64_t e, const uint64_t* row
  * q, out: BF16 [n_q][heads * dim]; k, v: BF16 [n_k][kv_heads * dim]; query head
  * h reads key head h / (heads / kv_heads). ld* are row strides in elements;
  * rows 16-byte aligned. lse: FP32 [n_q][heads] or NULL. slopes: FP32 [heads].
- * dim: a multiple of 8, at most 128 (GAT_B200_EUNSUPPORTED otherwise). scale in
+ * dim: a multiple of 8, at most 128 (GAT_B200_EUNSUPPORTED otherwise). What is
+ * written overlaps nothing that is read. scale in
  * (0, 1e30], cap in [0, 1e30]. Scores
  * and sums are FP32; the weights are rounded to BF16 for the second product, and
  * taken relative to a fixed score (cap up to 55) or to a maximum that follows
